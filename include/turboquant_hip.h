@@ -641,6 +641,90 @@ int tq_core_rotation(int32_t dim, int32_t seed, float* out);
 int tq_core_codebook(int32_t bits, int32_t dim, float* boundaries, float* centroids);
 
 /*
+ * A serving step's batch metadata, made on the GPU from device lengths (the reference's vLLM
+ * backend takes whatever the scheduler holds on the host and ignores it, vllm_plugin/
+ * __init__.py:350-412).  Requests r = 0 .. n_requests - 1 (at most 8192) hold context_lens[r]
+ * tokens and bring new_lens[r] more (negative: 0).  Tokens are laid out request after request;
+ * past n_tokens none are taken.
+ *   tq_paged_batch_plan: block j of request r (tokens j * block_size ..) that its context does
+ *     not reach yet takes the next of free_blocks [n_free], counted from *free_start (null: 0),
+ *     in request order, and is stored in block_tables [n_requests][table_stride] (its first
+ *     max_blocks entries count); entries of blocks the request holds are only read, others
+ *     stay as they were.  query_start_loc [n_requests + 1], seq_lens [n_requests] (context and
+ *     new tokens); per token i of n_tokens: slot_mapping (table entry * block_size + position
+ *     % block_size; -1 past the last request, past the table, and where no block is left or
+ *     the entry is negative), positions (0 past the last request) and token_request (-1
+ *     there); blocks_used [1]: the blocks the step needs, more than n_free - *free_start if
+ *     the free list was too short (the entries then hold -1).
+ *   tq_shared_prefix_groups: neighbouring requests whose tables begin with the same blocks.
+ *     Requests r - 1 and r join if the equal leading entries, of the blocks that lie wholly
+ *     inside both contexts (and are not negative), cover min_tokens >= 1 tokens or more; a
+ *     group is a maximal run of joined requests.  group_start_loc [n_requests + 1] gets each
+ *     group's first request, then n_requests; shared_lens [n_requests] the tokens all of a
+ *     group's tables begin with (the least over its neighbours; 0 for single requests and
+ *     behind the last group): the arguments of tq_attention_batch_paged_dl.
+ */
+int tq_paged_batch_plan(const int32_t* new_lens, const int32_t* context_lens, int32_t n_requests,
+                        int32_t* block_tables, int64_t table_stride, int32_t max_blocks,
+                        const int32_t* free_blocks, int64_t n_free, const int32_t* free_start,
+                        int32_t block_size, int32_t n_tokens, int32_t* query_start_loc,
+                        int32_t* seq_lens, int64_t* slot_mapping, int64_t* positions,
+                        int32_t* token_request, int32_t* blocks_used, void* stream);
+size_t tq_shared_prefix_groups_workspace_bytes(int32_t n_requests);
+int tq_shared_prefix_groups(const int32_t* block_tables, int64_t table_stride, int32_t max_blocks,
+                            const int32_t* context_lens, int32_t n_requests, int32_t block_size,
+                            int32_t min_tokens, int32_t* group_start_loc, int32_t* shared_lens,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
+/* How scores are changed and which positions a query sees (zeros and nulls: not at all). */
+typedef struct tq_score_variant {
+  float softcap;               /* scores become softcap * tanh(score / softcap); 0: off */
+  const float* alibi_slopes;   /* [hq]: + slope * (key position - query position) */
+  int32_t window;              /* the last `window` positions, the query's own included; 0: all */
+  const int32_t* prefix_lens;  /* [n_seqs]: all tokens of a sequence see its first prefix_lens */
+  const int32_t* token_starts; /* [n_tokens]: the first position each token sees */
+} tq_score_variant;
+
+/*
+ * Attention of a ragged batch over decode-layout paged pools (those of
+ * tq_decode_attention_paged_dl): prompts, chunks and single tokens in any mix, lengths on the
+ * device.  Sequence b's new tokens are rows query_start_loc[b] .. query_start_loc[b + 1] - 1 of
+ * q [n_tokens][hq][64] (q_stride elements between tokens; 16-byte aligned, strides too), the
+ * last ones of its seq_lens[b] tokens, read through block_tables [n_seqs][table_stride] (its
+ * first max_blocks entries).  A token at position p sees the positions
+ *   max(token_start, p - window + 1) <= j < min(seq_len, max(p + 1, prefix_len)),
+ * a part that is not given not bounding; scores are scaled, then capped, then biased.  A token
+ * that sees nothing gets zeros (lse -inf).  out [n_tokens][hq][64] in q_dtype (out_stride
+ * elements between tokens), lse [n_tokens][hq] fp32 or null (natural log).  Rows behind the
+ * last sequence keep out's values (zero_tail != 0: get zeros); their lse is -inf.
+ * With groups (n_groups > 0; group_start_loc [n_groups + 1] sequences, ascending; shared_lens
+ * [n_groups]): the tables of a group's sequences all begin with the blocks of its first
+ * shared_lens tokens, which are then read once for all the group's rows, through its first
+ * sequence's table.  Results are those without groups, to rounding.
+ * Replaces the reference backend's attention (vllm_plugin/__init__.py:400), whose Impl takes
+ * alibi_slopes, sliding_window and logits_soft_cap and applies none of them.
+ * Positions past max_blocks * block_size hold no tokens; block ids are clamped into the pool.
+ * workspace: tq_attention_batch_workspace_bytes(.., capacity = max_blocks * block_size) bytes,
+ * 16-byte aligned; calls that may run at the same time need one each.
+ */
+size_t tq_attention_batch_workspace_bytes(tq_dtype q_dtype, int32_t n_tokens, int32_t hq,
+                                          int32_t hkv, int32_t n_seqs, int32_t n_groups,
+                                          int64_t capacity);
+int tq_attention_batch_paged_dl(const void* q, tq_dtype q_dtype, int32_t n_tokens, int64_t q_stride,
+                                int32_t hq, int32_t hkv, int32_t d, const uint8_t* kpairs_pool,
+                                const float* knorm_pool, const uint8_t* vtile_pool,
+                                const float* vnorm_pool, int64_t num_blocks, int32_t block_size,
+                                int32_t vbits, const int32_t* block_tables, int64_t table_stride,
+                                int32_t max_blocks, const int32_t* query_start_loc,
+                                const int32_t* seq_lens, int32_t n_seqs,
+                                const int32_t* group_start_loc, const int32_t* shared_lens,
+                                int32_t n_groups, const float* kcentroids, const float* vcentroids,
+                                const float* krotation, const float* vrotation, float scale,
+                                const tq_score_variant* variant, void* out, int64_t out_stride,
+                                int32_t zero_tail, float* lse, void* workspace,
+                                size_t workspace_bytes, void* stream);
+
+/*
  * Huffman streams of code indices (host memory; the byte format of HuffmanCoder.encode /
  * decode, turboquant_kv/entropy.py:162-231): uint32 LE symbol count, uint32 LE bit count,
  * then the code words most significant bit first, zero-padded to a byte.  The caller

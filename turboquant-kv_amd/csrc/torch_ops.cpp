@@ -1221,6 +1221,220 @@ void prefill_attention_paged_dl_out(
                    krotation, vrotation, scale, out);
 }
 
+// ------------------------------------------------------------ batch metadata
+
+at::Tensor int32c(const at::Tensor& t, const at::Device& dev, const char* name) {
+  TORCH_CHECK(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, name, " must hold 32- or 64-bit integers");
+  return t.to(dev, at::kInt).contiguous();
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> paged_batch_plan(
+    const at::Tensor& new_lens, const at::Tensor& context_lens, at::Tensor& block_tables,
+    const at::Tensor& free_blocks, int64_t block_size, int64_t num_tokens,
+    const c10::optional<at::Tensor>& free_start) {
+  require_gpu(block_tables, "block_tables");
+  c10::DeviceGuard g(block_tables.device());
+  const auto dev = block_tables.device();
+  auto nl = int32c(new_lens, dev, "new_lens");
+  auto cl = int32c(context_lens, dev, "context_lens");
+  auto fb = int32c(free_blocks, dev, "free_blocks");
+  const int64_t R = nl.numel();
+  TORCH_CHECK(nl.dim() == 1 && cl.dim() == 1 && cl.numel() == R, "new_lens and context_lens must be [requests]");
+  TORCH_CHECK(fb.dim() == 1, "free_blocks must be one-dimensional");
+  TORCH_CHECK(block_tables.scalar_type() == at::kInt && block_tables.dim() == 2 && block_tables.size(0) == R &&
+                  (block_tables.size(1) <= 1 || block_tables.stride(1) == 1) &&
+                  (R <= 1 || block_tables.stride(0) >= block_tables.size(1)),
+              "block_tables is written in place: int32 [requests, max_blocks], its rows contiguous and apart");
+  TORCH_CHECK(block_size >= 1 && block_size <= INT32_MAX, "block_size must be positive, got ", block_size);
+  TORCH_CHECK(num_tokens >= 0 && num_tokens <= INT32_MAX, "num_tokens must be 0 or more, got ", num_tokens);
+  TORCH_CHECK(R <= INT32_MAX && block_tables.size(1) <= INT32_MAX, "too many requests or blocks");
+  at::Tensor fs;
+  if (free_start.has_value()) {
+    TORCH_CHECK(free_start->numel() == 1, "free_start must hold one value");
+    fs = int32c(*free_start, dev, "free_start");
+  }
+  const auto i32 = at::TensorOptions().dtype(at::kInt).device(dev);
+  const auto i64 = i32.dtype(at::kLong);
+  auto qs = at::empty({R + 1}, i32), sl = at::empty({R}, i32), sm = at::empty({num_tokens}, i64);
+  auto pos = at::empty({num_tokens}, i64), tr = at::empty({num_tokens}, i32), used = at::empty({1}, i32);
+  check_rc(tq_paged_batch_plan(nl.data_ptr<int32_t>(), cl.data_ptr<int32_t>(), (int32_t)R,
+                               block_tables.data_ptr<int32_t>(), R <= 1 ? block_tables.size(1) : block_tables.stride(0),
+                               (int32_t)block_tables.size(1), fb.data_ptr<int32_t>(), fb.numel(),
+                               fs.defined() ? fs.data_ptr<int32_t>() : nullptr, (int32_t)block_size,
+                               (int32_t)num_tokens, qs.data_ptr<int32_t>(), sl.data_ptr<int32_t>(),
+                               sm.data_ptr<int64_t>(), pos.data_ptr<int64_t>(), tr.data_ptr<int32_t>(),
+                               used.data_ptr<int32_t>(), cur_stream(block_tables)));
+  return {qs, sl, sm, pos, tr, used};
+}
+
+std::tuple<at::Tensor, at::Tensor> shared_prefix_groups(const at::Tensor& block_tables, const at::Tensor& context_lens,
+                                                        int64_t block_size, int64_t min_tokens) {
+  require_gpu(block_tables, "block_tables");
+  TORCH_CHECK(block_tables.dim() == 2, "block_tables must be [requests, max_blocks]");
+  c10::DeviceGuard g(block_tables.device());
+  const auto dev = block_tables.device();
+  auto bt = int32c(block_tables, dev, "block_tables");
+  auto cl = int32c(context_lens, dev, "context_lens");
+  const int64_t R = bt.size(0);
+  TORCH_CHECK(cl.dim() == 1 && cl.numel() == R, "context_lens must be [requests]");
+  TORCH_CHECK(block_size >= 1 && block_size <= INT32_MAX, "block_size must be positive, got ", block_size);
+  TORCH_CHECK(min_tokens >= 1 && min_tokens <= INT32_MAX, "min_tokens must be positive, got ", min_tokens);
+  TORCH_CHECK(R <= INT32_MAX && bt.size(1) <= INT32_MAX, "too many requests or blocks");
+  auto starts = at::empty({R + 1}, bt.options()), shared = at::empty({R}, bt.options());
+  auto ws = workspace(tq_shared_prefix_groups_workspace_bytes((int32_t)R), dev);
+  check_rc(tq_shared_prefix_groups(bt.data_ptr<int32_t>(), bt.size(1), (int32_t)bt.size(1), cl.data_ptr<int32_t>(),
+                                   (int32_t)R, (int32_t)block_size, (int32_t)min_tokens, starts.data_ptr<int32_t>(),
+                                   shared.data_ptr<int32_t>(), ws.data_ptr(), ws.numel(), cur_stream(bt)));
+  return {starts, shared};
+}
+
+// ------------------------------------------------------------ ragged batch attention
+
+// Queries or outputs the kernels read and write in place: heads and dims contiguous, tokens at
+// any stride of whole 16-byte units.
+bool token_rows(const at::Tensor& t) {
+  const int64_t esz = t.element_size();
+  return (t.size(2) <= 1 || t.stride(2) == 1) && (t.size(1) <= 1 || t.stride(1) == t.size(2)) &&
+         (t.size(0) <= 1 || (t.stride(0) >= t.size(1) * t.size(2) && t.stride(0) * esz % 16 == 0)) &&
+         reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+}
+
+std::tuple<at::Tensor, at::Tensor> attention_batch(
+    const at::Tensor& q, const at::Tensor& kpairs_pool, const at::Tensor& knorm_pool,
+    const at::Tensor& vtile_pool, const at::Tensor& vnorm_pool, const at::Tensor& block_tables,
+    const at::Tensor& query_start_loc, const at::Tensor& seq_lens,
+    const c10::optional<at::Tensor>& group_start_loc, const c10::optional<at::Tensor>& shared_lens,
+    const at::Tensor& kcentroids, const at::Tensor& vcentroids, const at::Tensor& krotation,
+    const at::Tensor& vrotation, double scale, double softcap, const c10::optional<at::Tensor>& alibi_slopes,
+    int64_t window, const c10::optional<at::Tensor>& prefix_lens, const c10::optional<at::Tensor>& token_starts,
+    bool want_lse, const c10::optional<at::Tensor>& into) {
+  require_gpu(q, "q");
+  TORCH_CHECK(q.dim() == 3, "q must be [num_tokens, Hq, d]");
+  TORCH_CHECK(kpairs_pool.dim() == 4 && vtile_pool.dim() == 4,
+              "kpairs_pool must be [num_blocks, hkv, block_size, d/2] and vtile_pool "
+              "[num_blocks, hkv, block_size/64, 512 VB]");
+  c10::DeviceGuard g(q.device());
+  const auto dev = q.device();
+  TORCH_CHECK(q.scalar_type() == at::kFloat || q.scalar_type() == at::kHalf || q.scalar_type() == at::kBFloat16,
+              "q must be float32, float16 or bfloat16");
+  const auto qq = token_rows(q) ? q : q.clone(at::MemoryFormat::Contiguous);
+  const int64_t n = qq.size(0), Hq = qq.size(1), d = qq.size(2);
+  const int64_t nb = kpairs_pool.size(0), Hkv = kpairs_pool.size(1), bs = kpairs_pool.size(2);
+  TORCH_CHECK(d == 64, "decode layout covers head_dim 64, got ", d);
+  for (const at::Tensor* t : {&kpairs_pool, &vtile_pool, &knorm_pool, &vnorm_pool})
+    TORCH_CHECK(t->device() == dev && t->is_contiguous(), "pools must be contiguous on the query's device");
+  TORCH_CHECK(kpairs_pool.scalar_type() == at::kByte && vtile_pool.scalar_type() == at::kByte,
+              "pools must be uint8");
+  const int64_t tile_tokens = bs >= 64 ? 64 : 16;
+  const int vb = value_tile_bits(vtile_pool.size(3), bs >= 64);
+  TORCH_CHECK(kpairs_pool.size(3) == d / 2 && vtile_pool.size(0) == nb && vtile_pool.size(1) == Hkv &&
+                  vtile_pool.size(2) * tile_tokens == bs && vb != 0,
+              "decode-layout pool shapes mismatch: value tiles [num_blocks, hkv, block_size/64, "
+              "512 VB] (block_size >= 64) or [num_blocks, hkv, block_size/16, 128 VB] (block_size "
+              "16, 32), VB = 2-4 value bits, head_dim 64");
+  TORCH_CHECK(knorm_pool.scalar_type() == at::kFloat && vnorm_pool.scalar_type() == at::kFloat &&
+                  knorm_pool.numel() == nb * Hkv * bs && vnorm_pool.numel() == nb * Hkv * bs,
+              "norm pools must be float32 [num_blocks, hkv, block_size]");
+  auto bt = int32c(block_tables, dev, "block_tables");
+  auto sl = int32c(seq_lens, dev, "seq_lens");
+  auto qs = int32c(query_start_loc, dev, "query_start_loc");
+  const int64_t B = sl.numel();
+  TORCH_CHECK(bt.dim() == 2 && bt.size(0) == B, "block_tables must be [num_seqs, max_blocks]");
+  TORCH_CHECK(qs.numel() == B + 1, "query_start_loc must have num_seqs + 1 entries");
+  auto kc = f32c(kcentroids, dev);
+  auto vc = f32c(vcentroids, dev);
+  auto Rk = f32c(krotation, dev);
+  auto Rv = f32c(vrotation, dev);
+  TORCH_CHECK(kc.numel() == 16 && vc.numel() == (1 << vb),
+              "decode layout: 4-bit keys (16 centroids) and 2^VB value centroids for the pool's "
+              "VB-bit value tiles");
+  TORCH_CHECK(Rk.numel() == d * d && Rv.numel() == d * d, "rotations must be [d, d]");
+  TORCH_CHECK(softcap >= 0 && std::isfinite(softcap), "softcap must be finite and not negative, got ", softcap);
+  TORCH_CHECK(window >= 0, "window must not be negative, got ", window);
+  TORCH_CHECK(n <= INT32_MAX && B < INT32_MAX && Hq <= INT32_MAX && bt.size(1) <= INT32_MAX, "too many tokens");
+  tq_score_variant v{};
+  v.softcap = (float)softcap;
+  v.window = (int32_t)std::min<int64_t>(window, INT32_MAX);
+  at::Tensor slopes, prefix, tstarts, groups, shared;
+  if (alibi_slopes.has_value()) {
+    TORCH_CHECK(alibi_slopes->numel() == Hq, "alibi_slopes must have one entry per query head");
+    slopes = f32c(*alibi_slopes, dev);
+    v.alibi_slopes = slopes.data_ptr<float>();
+  }
+  if (prefix_lens.has_value()) {
+    TORCH_CHECK(prefix_lens->numel() == B, "prefix_lens must have num_seqs entries");
+    prefix = int32c(*prefix_lens, dev, "prefix_lens");
+    v.prefix_lens = prefix.data_ptr<int32_t>();
+  }
+  if (token_starts.has_value()) {
+    TORCH_CHECK(token_starts->numel() == n, "token_starts must have one entry per token of q");
+    tstarts = int32c(*token_starts, dev, "token_starts");
+    v.token_starts = tstarts.data_ptr<int32_t>();
+  }
+  TORCH_CHECK(group_start_loc.has_value() == shared_lens.has_value(), "group_start_loc and shared_lens come together");
+  int64_t ng = 0;
+  if (group_start_loc.has_value()) {
+    groups = int32c(*group_start_loc, dev, "group_start_loc");
+    shared = int32c(*shared_lens, dev, "shared_lens");
+    ng = shared.numel();
+    TORCH_CHECK(groups.numel() == ng + 1, "group_start_loc must have one entry more than shared_lens");
+    TORCH_CHECK(ng <= INT32_MAX, "too many groups");
+  }
+  if (into.has_value())
+    TORCH_CHECK(into->device() == dev && into->sizes() == qq.sizes() && into->scalar_type() == qq.scalar_type() &&
+                    token_rows(*into),
+                "out must have the query's shape, dtype and device, heads contiguous, tokens 16-byte aligned");
+  auto out = into.has_value() ? *into : at::empty({n, Hq, d}, qq.options());
+  auto lse = want_lse ? at::empty({n, Hq}, qq.options().dtype(at::kFloat)) : at::Tensor();
+  if (n == 0 || Hq == 0) return {out, lse};
+  auto ws = workspace(tq_attention_batch_workspace_bytes(to_tq(qq.scalar_type()), (int32_t)n, (int32_t)Hq, (int32_t)Hkv,
+                                                         (int32_t)B, (int32_t)ng, bt.size(1) * bs),
+                      dev);
+  check_rc(tq_attention_batch_paged_dl(
+      qq.data_ptr(), to_tq(qq.scalar_type()), (int32_t)n, n <= 1 ? Hq * d : qq.stride(0), (int32_t)Hq, (int32_t)Hkv,
+      (int32_t)d, kpairs_pool.data_ptr<uint8_t>(), knorm_pool.data_ptr<float>(), vtile_pool.data_ptr<uint8_t>(),
+      vnorm_pool.data_ptr<float>(), nb, (int32_t)bs, (int32_t)vb, bt.data_ptr<int32_t>(), bt.size(1),
+      (int32_t)bt.size(1), qs.data_ptr<int32_t>(), sl.data_ptr<int32_t>(), (int32_t)B,
+      ng ? groups.data_ptr<int32_t>() : nullptr, ng ? shared.data_ptr<int32_t>() : nullptr, (int32_t)ng,
+      kc.data_ptr<float>(), vc.data_ptr<float>(), Rk.data_ptr<float>(), Rv.data_ptr<float>(), (float)scale, &v,
+      out.data_ptr(), n <= 1 ? Hq * d : out.stride(0), into.has_value() ? 0 : 1,
+      want_lse ? lse.data_ptr<float>() : nullptr, ws.data_ptr(), ws.numel(), cur_stream(qq)));
+  return {out, lse};
+}
+
+std::tuple<at::Tensor, at::Tensor> attention_batch_paged_dl(
+    const at::Tensor& q, const at::Tensor& kpairs_pool, const at::Tensor& knorm_pool,
+    const at::Tensor& vtile_pool, const at::Tensor& vnorm_pool, const at::Tensor& block_tables,
+    const at::Tensor& query_start_loc, const at::Tensor& seq_lens,
+    const c10::optional<at::Tensor>& group_start_loc, const c10::optional<at::Tensor>& shared_lens,
+    const at::Tensor& kcentroids, const at::Tensor& vcentroids, const at::Tensor& krotation,
+    const at::Tensor& vrotation, double scale, double softcap, const c10::optional<at::Tensor>& alibi_slopes,
+    int64_t window, const c10::optional<at::Tensor>& prefix_lens, const c10::optional<at::Tensor>& token_starts,
+    bool want_lse) {
+  auto r = attention_batch(q, kpairs_pool, knorm_pool, vtile_pool, vnorm_pool, block_tables, query_start_loc, seq_lens,
+                           group_start_loc, shared_lens, kcentroids, vcentroids, krotation, vrotation, scale, softcap,
+                           alibi_slopes, window, prefix_lens, token_starts, want_lse, c10::nullopt);
+  if (!want_lse) std::get<1>(r) = at::empty({0}, std::get<0>(r).options().dtype(at::kFloat));
+  return r;
+}
+
+// The same into `out`; rows behind the last sequence keep their values.
+at::Tensor attention_batch_paged_dl_out(
+    const at::Tensor& q, const at::Tensor& kpairs_pool, const at::Tensor& knorm_pool,
+    const at::Tensor& vtile_pool, const at::Tensor& vnorm_pool, const at::Tensor& block_tables,
+    const at::Tensor& query_start_loc, const at::Tensor& seq_lens,
+    const c10::optional<at::Tensor>& group_start_loc, const c10::optional<at::Tensor>& shared_lens,
+    const at::Tensor& kcentroids, const at::Tensor& vcentroids, const at::Tensor& krotation,
+    const at::Tensor& vrotation, double scale, double softcap, const c10::optional<at::Tensor>& alibi_slopes,
+    int64_t window, const c10::optional<at::Tensor>& prefix_lens, const c10::optional<at::Tensor>& token_starts,
+    bool want_lse, at::Tensor& out) {
+  auto lse = std::get<1>(attention_batch(q, kpairs_pool, knorm_pool, vtile_pool, vnorm_pool, block_tables,
+                                         query_start_loc, seq_lens, group_start_loc, shared_lens, kcentroids, vcentroids,
+                                         krotation, vrotation, scale, softcap, alibi_slopes, window, prefix_lens,
+                                         token_starts, want_lse, out));
+  return want_lse ? lse : at::empty({0}, out.options().dtype(at::kFloat));
+}
+
 // Every sequence's first `length` tokens.
 at::Tensor decode_attention_dl_len(const at::Tensor& q, const at::Tensor& kpairs,
                                    const at::Tensor& knorms, const at::Tensor& vblocks,
@@ -1549,6 +1763,20 @@ TORCH_LIBRARY(turboquant, m) {
         " Tensor vtile_pool, Tensor vnorm_pool, Tensor block_tables, Tensor seq_lens,"
         " Tensor kcentroids, Tensor vcentroids, Tensor krotation, Tensor vrotation,"
         " float scale) -> (Tensor, Tensor)");
+  m.def("paged_batch_plan(Tensor new_lens, Tensor context_lens, Tensor(a!) block_tables, Tensor free_blocks,"
+        " int block_size, int num_tokens, Tensor? free_start) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def("shared_prefix_groups(Tensor block_tables, Tensor context_lens, int block_size, int min_tokens)"
+        " -> (Tensor, Tensor)");
+  m.def("attention_batch_paged_dl(Tensor q, Tensor kpairs_pool, Tensor knorm_pool,"
+        " Tensor vtile_pool, Tensor vnorm_pool, Tensor block_tables, Tensor query_start_loc, Tensor seq_lens,"
+        " Tensor? group_start_loc, Tensor? shared_lens, Tensor kcentroids, Tensor vcentroids,"
+        " Tensor krotation, Tensor vrotation, float scale, float softcap, Tensor? alibi_slopes, int window,"
+        " Tensor? prefix_lens, Tensor? token_starts, bool want_lse) -> (Tensor, Tensor)");
+  m.def("attention_batch_paged_dl_out(Tensor q, Tensor kpairs_pool, Tensor knorm_pool,"
+        " Tensor vtile_pool, Tensor vnorm_pool, Tensor block_tables, Tensor query_start_loc, Tensor seq_lens,"
+        " Tensor? group_start_loc, Tensor? shared_lens, Tensor kcentroids, Tensor vcentroids,"
+        " Tensor krotation, Tensor vrotation, float scale, float softcap, Tensor? alibi_slopes, int window,"
+        " Tensor? prefix_lens, Tensor? token_starts, bool want_lse, Tensor(a!) out) -> Tensor");
   m.def("prefill_attention_paged_dl(Tensor q, Tensor kpairs_pool, Tensor knorm_pool,"
         " Tensor vtile_pool, Tensor vnorm_pool, Tensor block_table, int T,"
         " Tensor kcentroids, Tensor vcentroids, Tensor krotation, Tensor vrotation,"
@@ -1583,6 +1811,10 @@ TORCH_LIBRARY_IMPL(turboquant, CUDA, m) {
   m.impl("paged_store_value_tiles", &paged_store_value_tiles);
   m.impl("paged_write_dl", &paged_write_dl);
   m.impl("decode_attention_paged_dl", &decode_attention_paged_dl);
+  m.impl("paged_batch_plan", &paged_batch_plan);
+  m.impl("shared_prefix_groups", &shared_prefix_groups);
+  m.impl("attention_batch_paged_dl", &attention_batch_paged_dl);
+  m.impl("attention_batch_paged_dl_out", &attention_batch_paged_dl_out);
   m.impl("prefill_attention_paged_dl", &prefill_attention_paged_dl);
   m.impl("prefill_attention_paged_dl_out", &prefill_attention_paged_dl_out);
   m.impl("attention_scores_prod", &attention_scores_prod);

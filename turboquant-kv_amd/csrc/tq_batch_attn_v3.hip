@@ -1,0 +1,6 @@
+// tq_batch_attn_v3.hip -- the batch attention kernels for 3-bit values.
+#include "tq_batch_attn_kernel.h"
+
+namespace tq {
+template void ba_launch<3>(const BaArgs&, bool, bool, bool, int, unsigned, hipStream_t);
+}  // namespace tq

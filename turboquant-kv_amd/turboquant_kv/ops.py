@@ -247,3 +247,92 @@ def prefill_attention_paged_dl(q, kpairs_pool, knorm_pool, vtile_pool, vnorm_poo
     return _ops().prefill_attention_paged_dl(q, kpairs_pool, knorm_pool, vtile_pool, vnorm_pool,
                                              block_table, int(T), kcentroids, vcentroids,
                                              krotation, vrotation, float(scale))
+
+
+def paged_batch_plan(new_lens, context_lens, block_tables, free_blocks, block_size, num_tokens,
+                     free_start=None):
+    """A step's block tables and slot map from the requests' lengths, on the GPU.
+
+    Request r holds context_lens[r] tokens and brings new_lens[r] more, laid out request after
+    request in num_tokens token rows (more than their sum: padding; fewer: the rest is left
+    out).  Blocks that a request's context does not reach yet come from free_blocks, counted
+    from free_start (a one-element tensor; 0 without it), in request order, and are written
+    into block_tables [requests, max_blocks] (int32, in place; other entries stay).  At most
+    8192 requests.
+
+    -> query_start_loc [requests + 1], seq_lens [requests] (int32); slot_mapping (int64; -1
+    for padding, past the table's width, and where no block is left), positions (int64) and
+    token_request (int32; -1 for padding), each [num_tokens]; blocks_used [1] (int32): the
+    blocks the step needs -- more than the free list holds if it was too short, and the
+    entries that found none are -1."""
+    _require_device(block_tables, "block_tables")
+    return _ops().paged_batch_plan(new_lens, context_lens, block_tables, free_blocks,
+                                   int(block_size), int(num_tokens), free_start)
+
+
+def shared_prefix_groups(block_tables, context_lens, block_size, min_tokens=256):
+    """Neighbouring requests whose block tables begin with the same blocks.
+
+    Requests r - 1 and r join where their equal leading entries, of the blocks that lie wholly
+    inside both contexts, cover at least min_tokens tokens; a group is a maximal run of joined
+    requests and shares what all its neighbours do.  -> group_start_loc [requests + 1] (the
+    first request of each group, then the number of requests) and shared_lens [requests] (0
+    for single requests and behind the last group), int32: the arguments of
+    attention_shared_prefix_paged_dl."""
+    _require_device(block_tables, "block_tables")
+    return _ops().shared_prefix_groups(block_tables, context_lens, int(block_size), int(min_tokens))
+
+
+def _attention_batch(q, pools, block_tables, query_start_loc, seq_lens, groups, tables, scale, softcap,
+                     alibi_slopes, window, prefix_lens, token_starts, out, return_lse):
+    _require_device(q, "q")
+    args = (q, *pools, block_tables, query_start_loc, seq_lens, *groups, *tables, float(scale), float(softcap),
+            alibi_slopes, int(window), prefix_lens, token_starts, bool(return_lse))
+    if out is None:
+        out, lse = _ops().attention_batch_paged_dl(*args)
+    else:
+        lse = _ops().attention_batch_paged_dl_out(*args, out)
+    return (out, lse) if return_lse else out
+
+
+def attention_batch_paged_dl(q, kpairs_pool, knorm_pool, vtile_pool, vnorm_pool, block_tables,
+                             query_start_loc, seq_lens, kcentroids, vcentroids, krotation, vrotation,
+                             scale, *, softcap=0.0, alibi_slopes=None, window=0, prefix_lens=None,
+                             token_starts=None, out=None, return_lse=False):
+    """Attention of a ragged batch over decode-layout paged pools (head_dim 64): prompts, chunks
+    and single tokens in any mix, their lengths read on the device.
+
+    Sequence b's new tokens are rows query_start_loc[b] .. query_start_loc[b + 1] - 1 of
+    q [num_tokens, Hq, 64] (float32, float16 or bfloat16; any token stride) and the last ones
+    of its seq_lens[b] tokens.  A token at position p sees the positions
+        max(token_starts, p - window + 1) <= j < min(seq_len, max(p + 1, prefix_len)):
+    causal, within the last `window` positions (0: all), from token_starts [num_tokens] on (a
+    packed document's first token), and all of the first prefix_lens [num_seqs] positions,
+    later ones included.  Scores are scaled, capped (softcap * tanh(score / softcap); 0: not)
+    and biased (alibi_slopes [Hq] * (j - p)).
+
+    -> [num_tokens, Hq, 64] in q's dtype, zeros for rows that see nothing; with return_lse also
+    the [num_tokens, Hq] float32 log-sum-exp of the scores (-inf there).  Rows behind the last
+    sequence are zeros, or keep their values in a given `out` (which must not share q's memory).
+    For inference: no gradient flows through it."""
+    return _attention_batch(q, (kpairs_pool, knorm_pool, vtile_pool, vnorm_pool), block_tables,
+                            query_start_loc, seq_lens, (None, None),
+                            (kcentroids, vcentroids, krotation, vrotation), scale, softcap, alibi_slopes,
+                            window, prefix_lens, token_starts, out, return_lse)
+
+
+def attention_shared_prefix_paged_dl(q, kpairs_pool, knorm_pool, vtile_pool, vnorm_pool, block_tables,
+                                     query_start_loc, seq_lens, group_start_loc, shared_lens, kcentroids,
+                                     vcentroids, krotation, vrotation, scale, *, softcap=0.0,
+                                     alibi_slopes=None, window=0, prefix_lens=None, token_starts=None,
+                                     out=None, return_lse=False):
+    """attention_batch_paged_dl for batches whose sequences share a prefix: the sequences
+    group_start_loc[g] .. group_start_loc[g + 1] - 1 have block tables that begin with the same
+    blocks for their first shared_lens[g] tokens, and those are read once for all the group's
+    rows instead of once per sequence.  The results are attention_batch_paged_dl's, to rounding.
+    group_start_loc [groups + 1] ascends, shared_lens is [groups] (0: nothing shared); sequences
+    in no group are taken as they are.  shared_prefix_groups finds both."""
+    return _attention_batch(q, (kpairs_pool, knorm_pool, vtile_pool, vnorm_pool), block_tables,
+                            query_start_loc, seq_lens, (group_start_loc, shared_lens),
+                            (kcentroids, vcentroids, krotation, vrotation), scale, softcap, alibi_slopes,
+                            window, prefix_lens, token_starts, out, return_lse)
