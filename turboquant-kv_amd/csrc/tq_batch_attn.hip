@@ -1,5 +1,5 @@
 // tq_batch_attn.hip -- entry points of the ragged batch's attention (tq_batch_attn.h): the choice
-// of kernels, the workspace, and the kernel that joins the partial results.
+// of kernels and the workspace, the preparing kernel and the one that joins partial results.
 
 #include "tq_batch_attn.h"
 
@@ -8,87 +8,339 @@
 namespace tq {
 namespace {
 
-// Where a launch over the groups left its partial results.
-struct BaPrefix {
-  const float* slots;
-  const BaHead* head;
-  const BaItem* items;
-  const int32_t* seg_item;
-  const float* row_sums;
-  const float* row_stats;
-  int max_items;
-  int rows;  // of an item
+constexpr int kPrepThreads = 512;
+constexpr int kPrepWaves = kPrepThreads / 64;
+constexpr int kPrepStarts = 2048;  // items' places kept in LDS
+
+// ---------------------------------------------------------------------------- preparation
+
+// Exclusive sum over the workgroup; `all` gets the whole sum.
+__device__ __forceinline__ int64_t prep_scan(int64_t v, int64_t* part, int64_t* all) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int64_t incl = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int64_t up = __shfl_up(incl, o, 64);
+    if (lane >= o) incl += up;
+  }
+  __syncthreads();  // `part` may still be read from a scan before
+  if (lane == 63) part[wave] = incl;
+  __syncthreads();
+  int64_t before = 0, sum = 0;
+#pragma unroll
+  for (int w = 0; w < kPrepWaves; ++w) {
+    const int64_t p = part[w];
+    if (w < wave) before += p;
+    sum += p;
+  }
+  *all = sum;
+  return before + incl - v;
+}
+
+// Tokens of sequence b's context that its group's line covers.
+__device__ __forceinline__ int ba_shared(const BaArgs& a, int b) {
+  if (a.n_groups == 0) return 0;
+  const int g = ba_last(a.n_groups, b, [&](int i) { return a.group_start[i]; });
+  if (b < a.group_start[g] || b >= a.group_start[g + 1]) return 0;
+  return max(0, min(a.shared[g], a.cap));
+}
+
+// A segment of a line: the rows of a sequence or of a group's sequences, the positions the
+// line covers, and its table.
+struct BaSeg {
+  int tok0, ntok, lo, hi, table;
+  int past, prefix;  // sequences: the first token's position, prefix_lens
 };
 
-// Joins the partial results of 16 rows: those of an item cut between workgroups and, with
-// groups, the item's own and its group's.  The four waves take the sources in turn, then a
-// wave each rotates a quarter of the result's dims.  A row's sums of one source are 256
-// consecutive bytes; latency bounds it (a few microseconds).
-__global__ __launch_bounds__(256) void batch_combine_kernel(BaArgs a, BaPrefix p, int rows, int with_groups) {
+template <int L>
+__device__ __forceinline__ BaSeg ba_segment(const BaArgs& a, int s) {
+  BaSeg x{};
+  if (L == 1) {
+    const int b0 = max(0, min(a.group_start[s], a.B)), b1 = max(b0, min(a.group_start[s + 1], a.B));
+    x.hi = max(0, min(a.shared[s], a.cap));
+    if (b1 > b0 && x.hi > 0) {
+      x.tok0 = ba_qs(a, b0);
+      x.ntok = max(0, ba_qs(a, b1) - x.tok0);
+    }
+    x.table = max(0, min(b0, a.B - 1));
+  } else {
+    x.tok0 = ba_qs(a, s);
+    x.ntok = max(0, ba_qs(a, s + 1) - x.tok0);
+    const int T = max(0, a.seq_lens[s]);
+    x.past = T - x.ntok;
+    x.lo = ba_shared(a, s);
+    x.hi = min(T, a.cap);
+    x.prefix = a.prefix_lens ? a.prefix_lens[s] : 0;
+    x.table = s;
+  }
+  return x;
+}
+
+// Lays line L out: the items of every segment, their places, and the item that each wave's
+// piece begins in.
+template <int L>
+__device__ __forceinline__ void ba_lay_out(const BaArgs& a, int32_t* base_s, int64_t* start_s, int64_t* part) {
+  const BaLine& ln = a.line[L];
+  const int tid = threadIdx.x, R = ln.rows;
+  const int nseg = L == 1 ? a.n_groups : a.B;
+  // first items of the segments
+  int64_t run = 0;
+  for (int s0 = 0; s0 < nseg; s0 += kPrepThreads) {
+    const int s = s0 + tid;
+    int64_t n = 0, all;
+    if (s < nseg) n = ((int64_t)ba_segment<L>(a, s).ntok * a.G + R - 1) / R;
+    const int64_t at = prep_scan(n, part, &all);
+    if (s < nseg) base_s[s] = ln.seg_item[s] = (int)min<int64_t>(run + at, INT_MAX);
+    run += all;
+  }
+  if (tid == 0) base_s[nseg] = ln.seg_item[nseg] = (int)min<int64_t>(run, INT_MAX);
+  __syncthreads();
+  // (starts that do not ascend could make more items than there is room for)
+  const int n_items = min(base_s[nseg], ln.max_items);
+  int64_t place = 0;
+  for (int i0 = 0; i0 < n_items; i0 += kPrepThreads) {
+    const int i = i0 + tid;
+    int64_t cost = 0, all;
+    BaItem it{};
+    if (i < n_items) {
+      const int s = ba_last(nseg, i, [&](int k) { return base_s[k]; });
+      const BaSeg x = ba_segment<L>(a, s);
+      const int64_t row0 = (int64_t)(i - base_s[s]) * R;
+      it.tok0 = x.tok0;
+      it.row0 = (int)row0;
+      it.nrows = x.ntok * a.G;
+      it.table = x.table;
+      it.lo = x.lo;
+      it.hi = x.hi;
+      // Document starts bound single tokens; the waves of longer items skip the tiles that all
+      // their own rows' starts leave out.
+      int64_t lo = x.lo, hi = x.hi;
+      if (L == 0) {
+        const int i0t = (int)(row0 / a.G), i1t = min(x.ntok - 1, (int)((row0 + R - 1) / a.G));
+        hi = min<int64_t>(hi, max<int64_t>((int64_t)x.past + i1t + 1, x.prefix));
+        if (a.window > 0) lo = max<int64_t>(lo, (int64_t)x.past + i0t + 1 - a.window);
+        if (a.token_starts && x.ntok == 1 && hi > 0) lo = max<int64_t>(lo, a.token_starts[x.tok0]);
+      }
+      it.t0 = hi > lo ? (int)(lo >> 6) : 0;
+      it.nt = hi > lo ? (int)((hi + 63) >> 6) - it.t0 : 0;
+      cost = (int64_t)(it.nt + kBaOver) * a.hkv;
+    }
+    const int64_t at = prep_scan(cost, part, &all);
+    if (i < n_items) {
+      it.start = place + at;
+      ln.items[i] = it;
+      if (i < kPrepStarts) start_s[i] = it.start;
+    }
+    place += all;
+  }
+  // Equal pieces, of a few tiles at least.
+  const int64_t chunk = max<int64_t>(kBaOver + 1, (place + ln.waves - 1) / ln.waves);
+  if (tid == 0) *ln.head = BaHead{chunk, place, n_items, 0};
+  // the item that each wave's piece begins in
+  auto start_of = [&](int i) { return n_items <= kPrepStarts ? start_s[i] : ln.items[i].start; };
+  __syncthreads();
+  for (int w = tid; w < ln.waves; w += kPrepThreads) {
+    const int64_t p = w * chunk;
+    int lo = 0, hi = n_items;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (start_of(mid) <= p) lo = mid;
+      else hi = mid;
+    }
+    ln.work[w] = p < place ? lo : -1;
+  }
+}
+
+// Workgroups 0 .. n_lines - 1 lay the lines out; the others rotate 16 rows (a token's head
+// each) a wave: Qrot = (q * qscale) R_k^T by v_mfma_f32_16x16x4f32, scaled by a power of two
+// into [0.5, 1) and split into fp16 hi (and lo) parts, and find their tokens' positions.
+__global__ __launch_bounds__(kPrepThreads) void batch_prep_kernel(BaArgs a, int n_lines, int prec) {
 #pragma clang fp contract(off)
-  __shared__ __attribute__((aligned(16))) float sums_s[4][16][68];
-  __shared__ float stat_s[4][16][2];
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  __shared__ int32_t base_s[kBaMaxSegs + 2];
+  __shared__ int64_t start_s[kPrepStarts];
+  __shared__ int64_t part[kPrepWaves];
+  if ((int)blockIdx.x < n_lines) {
+    if (blockIdx.x == 0) ba_lay_out<0>(a, base_s, start_s, part);
+    else ba_lay_out<1>(a, base_s, start_s, part);
+    return;
+  }
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int c = lane & 15, g = lane >> 4;
-  const int ngr = rows / 16;
-  const int j = (int)(blockIdx.x % (unsigned)ngr);
-  const int h = (int)(blockIdx.x / (unsigned)ngr % (unsigned)a.hkv);
-  const int item = (int)(blockIdx.x / (unsigned)ngr / (unsigned)a.hkv);
-  if (item >= a.head->n_items) return;
-  const BaItem it = a.items[item];
-  const int64_t chunk = a.head->chunk, start = it.start + (int64_t)h * it.cost;
-  const int64_t w0 = start / chunk, w1 = (start + it.cost - 1) / chunk;
-  const bool cut = w1 > w0;
-  if (!with_groups && !cut) return;  // written by its workgroup
-  const BaSeg sg = ba_segment(a, it.seg, rows);
-  const int nrows = sg.ntok * a.G, irow = it.rt * rows + 16 * j;
-  if (irow >= nrows) return;
-  const int row = min(irow + c, nrows - 1);
-  const int ti = row / a.G, tok = sg.tok0 + ti, qh = h * a.G + (row - ti * a.G);
-  const int64_t rowid = (int64_t)tok * a.hq + qh;
-  const int ns = cut ? (int)(w1 - w0) + 1 : 1;
-  // the row's sources of its group's launch
-  int np = 0, prow = 0;
-  int64_t p0 = 0;
-  bool pcut = false;
-  if (with_groups && it.seg < a.B && a.n_groups > 0) {
-    const int gi = ba_last(a.n_groups, it.seg, [&](int i) { return a.group_start[i]; });
-    const int b0 = a.group_start[gi], b1 = min(a.group_start[gi + 1], a.B);
-    if (b0 >= 0 && it.seg >= b0 && it.seg < b1 && a.shared[gi] > 0) {
-      const int t0 = ba_qs(a, b0), t1 = ba_qs(a, b1);
-      if (tok >= t0 && tok < t1) {
-        const int64_t ro = (int64_t)(tok - t0) * a.G + (qh - h * a.G);
-        const BaItem pi = p.items[min(p.seg_item[gi] + (int)(ro / p.rows), p.max_items - 1)];
-        const int64_t pc = p.head->chunk, ps = pi.start + (int64_t)h * pi.cost;
-        prow = (int)(ro % p.rows);
-        p0 = ps / pc;
-        const int64_t p1 = (ps + pi.cost - 1) / pc;
-        pcut = p1 > p0;
-        np = (int)(p1 - p0) + 1;
+  const int64_t blk = (int)blockIdx.x - n_lines;
+  const int64_t n_rows = (int64_t)a.n_tokens * a.hq;
+  // ---- positions of token `t`
+  const int64_t t64 = blk * kPrepThreads + tid;
+  if (t64 < a.n_tokens) {
+    const int t = (int)t64;
+    BaToken x{0, 0, 0, a.B};
+    if (a.B > 0 && t >= ba_qs(a, 0) && t < ba_qs(a, a.B)) {
+      // token t of a step of single tokens belongs to sequence t
+      const int b = t < a.B && ba_qs(a, t) <= t && ba_qs(a, t + 1) > t
+                        ? t : ba_last(a.B, t, [&](int i) { return ba_qs(a, i); });
+      const int q0 = ba_qs(a, b), T = max(0, a.seq_lens[b]);
+      const int64_t p = (int64_t)T - (ba_qs(a, b + 1) - q0) + (t - q0);
+      int64_t lo = 0;
+      if (a.window > 0) lo = max<int64_t>(lo, p + 1 - a.window);
+      if (a.token_starts) lo = max<int64_t>(lo, a.token_starts[t]);
+      x.lo = (int)lo;
+      x.hi = (int)min<int64_t>(min(T, a.cap), max<int64_t>(p + 1, a.prefix_lens ? a.prefix_lens[b] : 0));
+      x.pos = (int)p;
+      x.seq = b;
+    }
+    a.tokens[t] = x;
+  }
+  // ---- rows.  MFMA mb, k-step s: lane (c, g) supplies A[c][g] = R_k[16 (c / 4) + 4 mb + c % 4][16 g + s]
+  // and B[g][c] = q_c[16 g + s]; register r of lane (c, g) gets Qrot_c[16 g + 4 mb + r]: a lane
+  // ends with dims 16 g .. 16 g + 15, the order in which its key bytes come.
+  const int64_t r0 = (blk * kPrepWaves + wave) * 16;
+  if (r0 >= n_rows) return;
+  const int64_t row = min(r0 + c, n_rows - 1);
+  const int64_t qo = row / a.hq * a.q_stride + row % a.hq * 64 + 16 * g;
+  float qv[16];
+  if (a.q_dt == TQ_F32) {
+    const ba_v4f* src = reinterpret_cast<const ba_v4f*>(static_cast<const float*>(a.q) + qo);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const ba_v4f v = src[i];
+      qv[4 * i] = v.x; qv[4 * i + 1] = v.y; qv[4 * i + 2] = v.z; qv[4 * i + 3] = v.w;
+    }
+  } else {
+    const ba_u32x4* src = reinterpret_cast<const ba_u32x4*>(static_cast<const uint16_t*>(a.q) + qo);
+    const bool bf = a.q_dt == TQ_BF16;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const ba_u32x4 v = src[i];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t hb = (v[e >> 1] >> (16 * (e & 1))) & 0xFFFFu;
+        qv[8 * i + e] = bf ? __uint_as_float(hb << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)hb);
       }
     }
   }
+  ba_v4f d[4];
+#pragma unroll
+  for (int mb = 0; mb < 4; ++mb) {
+    const ba_v4f* src = reinterpret_cast<const ba_v4f*>(a.krot + (16 * (c >> 2) + 4 * mb + (c & 3)) * 64 + 16 * g);
+    d[mb] = (ba_v4f){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const ba_v4f rk = src[i];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        d[mb] = __builtin_amdgcn_mfma_f32_16x16x4f32(rk[e], qv[4 * i + e] * a.qscale, d[mb], 0, 0, 0);
+    }
+  }
+  float qm = 0.f;
+#pragma unroll
+  for (int mb = 0; mb < 4; ++mb)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) qm = fmaxf(qm, fabsf(d[mb][r]));
+  qm = fmaxf(qm, __shfl_xor(qm, 16, 64));
+  qm = fmaxf(qm, __shfl_xor(qm, 32, 64));
+  int e = 0;
+  if (qm > 0.f && qm < INFINITY) frexpf(qm, &e);
+  const float qsc = ldexpf(1.f, -e);
+  ba_v8h hi[2], lo[2];
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float v = d[2 * s + (i >> 2)][i & 3] * qsc;
+      hi[s][i] = (_Float16)v;
+      lo[s][i] = (_Float16)(v - (float)hi[s][i]);
+    }
+  if (r0 + c >= n_rows) return;
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    *reinterpret_cast<ba_v8h*>(a.qhi + row * 64 + 16 * g + 8 * s) = hi[s];
+    if (prec) *reinterpret_cast<ba_v8h*>(a.qlo + row * 64 + 16 * g + 8 * s) = lo[s];
+  }
+  if (g == 0) a.qscale_inv[row] = ldexpf(1.f, e);
+}
+
+// ------------------------------------------------------------------------------- joining
+
+// Where one line left a row's sums: by row (one source), or in the slots of `count` waves
+// from w0 on.
+struct BaFrom {
+  int64_t w0;
+  int count, row;  // the row in its item
+  bool by_row;
+};
+
+__device__ __forceinline__ BaFrom ba_from(const BaArgs& a, const BaLine& ln, int seg, int64_t seg_row, int h) {
+  BaFrom f{};
+  const int n_items = ln.head->n_items;
+  if (n_items <= 0 || seg_row < 0) return f;
+  const BaItem it = ln.items[max(0, min(ln.seg_item[seg] + (int)(seg_row / ln.rows), n_items - 1))];
+  const int64_t chunk = ln.head->chunk;
+  const int cost = it.nt + kBaOver;
+  const int64_t start = it.start + (int64_t)h * cost;
+  f.row = (int)(seg_row % ln.rows);
+  // the waves that the first and the last tile fall to
+  f.w0 = (start + kBaOver) / chunk;
+  const int64_t w1 = (start + cost - 1) / chunk;
+  f.by_row = it.nt == 0 || f.w0 == w1;
+  f.count = f.by_row ? 1 : (int)(w1 - f.w0) + 1;
+  return f;
+}
+
+constexpr int kJoinWaves = 4;
+
+// 16 rows (a token's head each) per workgroup: a row's sums come from its sequence's line and,
+// with groups, from its group's.  The waves take a row's sources in turn, join theirs, then
+// wave ob rotates dims 16 ob .. of the whole back by R_v.  A source is 264 bytes of a row;
+// latency bounds it (a few microseconds).
+__global__ __launch_bounds__(64 * kJoinWaves) void batch_join_kernel(BaArgs a) {
+#pragma clang fp contract(off)
+  __shared__ __attribute__((aligned(16))) float sums_s[kJoinWaves][16][68];
+  __shared__ float stat_s[kJoinWaves][16][2];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  const int64_t n_rows = (int64_t)a.n_tokens * a.hq, r0 = (int64_t)blockIdx.x * 16;
+  const int64_t rowid = min(r0 + c, n_rows - 1);
+  const int tok = (int)(rowid / a.hq), qh = (int)(rowid - (int64_t)tok * a.hq);
+  const int h = qh / a.G, gq = qh - h * a.G;
+  // R_v's entries of this wave's dims, wanted last
+  float rv[16];
+#pragma unroll
+  for (int nb = 0; nb < 4; ++nb)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) rv[4 * nb + r] = a.vrot[(16 * nb + 4 * g + r) * 64 + 16 * wave + c];
+
+  const BaToken t = a.tokens[tok];
+  BaFrom s{}, p{};
+  if (t.seq < a.B) {
+    s = ba_from(a, a.line[0], t.seq, (int64_t)(tok - ba_qs(a, t.seq)) * a.G + gq, h);
+    if (a.n_groups > 0) {
+      const int gi = ba_last(a.n_groups, t.seq, [&](int i) { return a.group_start[i]; });
+      const int b0 = a.group_start[gi], b1 = min(a.group_start[gi + 1], a.B);
+      if (b0 >= 0 && t.seq >= b0 && t.seq < b1 && a.shared[gi] > 0 && a.cap > 0)
+        p = ba_from(a, a.line[1], gi, (int64_t)(tok - ba_qs(a, b0)) * a.G + gq, h);
+    }
+  }
+  const int ns = s.count, np = p.count;
   int most = ns + np;
 #pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) most = max(most, __shfl_xor(most, o, 64));
+  for (int o = 8; o >= 1; o >>= 1) most = max(most, __shfl_xor(most, o, 64));
+
   float m = -INFINITY, l = 0.f;
   ba_v4f o4[4];
 #pragma unroll
   for (int nb = 0; nb < 4; ++nb) o4[nb] = (ba_v4f){0.f, 0.f, 0.f, 0.f};
-  for (int i = wave; i < most; i += 4) {
-    const float *sums, *st;
+  for (int i = wave; i < most; i += kJoinWaves) {
     if (i >= ns + np) continue;
-    if (i < ns) {
-      const float* s = a.slots + ((w0 + i) * 2 + (i == 0)) * ba_slot_floats(rows);
-      sums = cut ? s + (16 * j + c) * 64 : a.row_sums + rowid * 64;
-      st = cut ? s + rows * 64 + (16 * j + c) * 2 : a.row_stats + rowid * 2;
-    } else {
-      const int k = i - ns;
-      const float* s = p.slots + ((p0 + k) * 2 + (k == 0)) * ba_slot_floats(p.rows);
-      sums = pcut ? s + prow * 64 : p.row_sums + rowid * 64;
-      st = pcut ? s + p.rows * 64 + prow * 2 : p.row_stats + rowid * 2;
-    }
+    const bool mine = i < ns;
+    const float *sums, *st;
+    auto source = [&](const BaLine& ln, const BaFrom& f, int k) {
+      // the wave with the item's first tile kept it in slot 1
+      const float* slot = ln.slots + ((f.w0 + k) * 2 + (k == 0)) * ba_slot_floats(ln.rows);
+      sums = f.by_row ? ln.row_sums + rowid * 64 : slot + f.row * 64;
+      st = f.by_row ? ln.row_stats + rowid * 2 : slot + ln.rows * 64 + f.row * 2;
+    };
+    if (mine) source(a.line[0], s, i);
+    else source(a.line[1], p, i - ns);
     const float mi = st[0], li = st[1];
     const float mn = fmaxf(m, mi), ms = mn == -INFINITY ? 0.f : mn;
     const float fa = __builtin_amdgcn_exp2f(m - ms), fb = __builtin_amdgcn_exp2f(mi - ms);
@@ -98,11 +350,6 @@ __global__ __launch_bounds__(256) void batch_combine_kernel(BaArgs a, BaPrefix p
     for (int nb = 0; nb < 4; ++nb)
       o4[nb] = o4[nb] * fa + *reinterpret_cast<const ba_v4f*>(sums + 16 * nb + 4 * g) * fb;
   }
-  float rv[16];  // R_v's entries of this wave's 16 dims, requested before the barrier
-#pragma unroll
-  for (int nb = 0; nb < 4; ++nb)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) rv[4 * nb + r] = a.vrot[(16 * nb + 4 * g + r) * 64 + 16 * wave + c];
 #pragma unroll
   for (int nb = 0; nb < 4; ++nb) *reinterpret_cast<ba_v4f*>(&sums_s[wave][c][16 * nb + 4 * g]) = o4[nb];
   if (g == 0) {
@@ -110,27 +357,29 @@ __global__ __launch_bounds__(256) void batch_combine_kernel(BaArgs a, BaPrefix p
     stat_s[wave][c][1] = l;
   }
   __syncthreads();
-  float M = -INFINITY, L = 0.f, f[4];
+  float M = -INFINITY, L = 0.f, f[kJoinWaves];
 #pragma unroll
-  for (int w = 0; w < 4; ++w) M = fmaxf(M, stat_s[w][c][0]);
+  for (int w = 0; w < kJoinWaves; ++w) M = fmaxf(M, stat_s[w][c][0]);
   const float Ms = M == -INFINITY ? 0.f : M;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
+  for (int w = 0; w < kJoinWaves; ++w) {
     f[w] = __builtin_amdgcn_exp2f(stat_s[w][c][0] - Ms);
     L += stat_s[w][c][1] * f[w];
   }
+  // out_c[16 ob + 4 g + r] of lane (c, g) = sum over k-steps (nb, r) of A[c][g] =
+  // R_v[16 nb + 4 g + r][16 ob + c] and B[g][c] = O_c[16 nb + 4 g + r]
   const float inv = L == 0.f ? 0.f : 1.f / L;
   ba_v4f acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int nb = 0; nb < 4; ++nb) {
     ba_v4f x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < 4; ++w) x += *reinterpret_cast<const ba_v4f*>(&sums_s[w][c][16 * nb + 4 * g]) * f[w];
+    for (int w = 0; w < kJoinWaves; ++w) x += *reinterpret_cast<const ba_v4f*>(&sums_s[w][c][16 * nb + 4 * g]) * f[w];
 #pragma unroll
     for (int r = 0; r < 4; ++r) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(rv[4 * nb + r], x[r] * inv, acc, 0, 0, 0);
   }
-  if (irow + c >= nrows) return;
-  if (it.seg < a.B || a.zero_tail) {
+  if (r0 + c >= n_rows) return;
+  if (t.seq < a.B || a.zero_tail) {
     const int64_t oa = (int64_t)tok * a.out_stride + qh * 64 + 16 * wave + 4 * g;
     if (a.q_dt == TQ_F32) {
       *reinterpret_cast<ba_v4f*>(static_cast<float*>(a.out) + oa) = acc;
@@ -146,68 +395,79 @@ __global__ __launch_bounds__(256) void batch_combine_kernel(BaArgs a, BaPrefix p
     a.lse[rowid] = L == 0.f ? -INFINITY : (M + __builtin_amdgcn_logf(L)) * 0.6931471805599453f;
 }
 
+// --------------------------------------------------------------------------------- plans
+
 // Which kernels a call runs, and its workspace.
 struct BaPlan {
-  bool prec, rows;   // rows: the row kernel
-  int groups, pgroups;  // row groups of a wave: sequences, prefix groups
-  int64_t items, pitems;
-  unsigned grid, pgrid;
-  size_t slots, pslots, row_bytes, total;
+  bool prec;
+  int rw[2], groups[2];  // per line: rows of a group of columns, groups
+  int64_t items[2];
+  unsigned grid[2];
+  int64_t segs[2];
 };
-
-constexpr size_t kBaHeadBytes = 256;
 
 BaPlan ba_plan(tq_dtype q_dtype, int64_t n, int hq, int hkv, int64_t B, int64_t n_groups, int64_t capacity) {
   BaPlan p{};
   p.prec = q_dtype != TQ_BF16;
-  const int most = ba_groups(p.prec), G = hq / hkv;
+  const int G = hq / hkv;
   const int64_t rows = n * G, cus = device_cu_count();
-  // One group of 16 rows a wave where sequences hold no more on average (a decode step);
-  // otherwise as many as the registers take, which share each tile's lookups.
-  p.groups = rows <= 16 * std::max<int64_t>(B, 1) ? 1 : most;
-  // Prompts whose rows alone fill the card go to the row kernel: nothing to merge.
-  p.rows = n_groups == 0 && p.groups > 1 && rows / (16 * most * kBaWaves) * hkv >= cus;
-  const int R = 16 * p.groups * (p.rows ? kBaWaves : 1);
-  p.items = rows / R + B + 1;
-  const int64_t tiles = capacity / 64 + 1;
-  auto split_grid = [&](int64_t items) {
-    const int64_t pieces = (items * hkv * tiles + kBaWaves - 1) / kBaWaves;
-    return (unsigned)std::max<int64_t>(1, std::min(cus, pieces));
-  };
-  p.grid = p.rows ? (unsigned)std::min<int64_t>(p.items * hkv, UINT_MAX) : split_grid(p.items);
-  size_t at = 0;
-  auto take = [&](size_t bytes) {
-    const size_t here = at;
-    at += align_up(bytes, 256);
-    return here;
-  };
-  if (!p.rows) {
-    take(kBaHeadBytes);
-    take(p.items * sizeof(BaItem));
-    p.slots = (size_t)p.grid * 2 * ba_slot_floats(16 * p.groups) * 4;
-    take(p.slots);
+  p.segs[0] = B;
+  p.segs[1] = n_groups;
+  for (int l = 0; l < (n_groups > 0 ? 2 : 1); ++l) {
+    // A group of columns as wide as a segment's rows are on average: single tokens of few heads
+    // use 4 or 8 of the 16 columns; rows beyond 16 share each tile's lookups.
+    // (whole tokens: a few rows of padding behind single tokens do not widen them)
+    const int64_t avg = std::max<int64_t>(1, n / std::max<int64_t>(l ? n_groups : B, 1)) * G;
+    p.rw[l] = avg <= 4 ? 4 : avg <= 8 ? 8 : 16;
+    p.groups[l] = avg <= 16 ? 1 : ba_groups(p.prec);
+    const int R = p.rw[l] * p.groups[l];
+    p.items[l] = rows / R + p.segs[l];
+    // one workgroup per CU, fewer where even one-tile pieces would not fill them
+    const int64_t pieces = p.items[l] * hkv * (capacity / 64 + 1 + kBaOver);
+    p.grid[l] = (unsigned)std::max<int64_t>(1, std::min(cus, pieces));
   }
-  if (n_groups > 0) {
-    p.pgroups = rows <= 16 * n_groups ? 1 : most;
-    p.pitems = rows / (16 * p.pgroups) + n_groups;
-    p.pgrid = split_grid(p.pitems);
-    p.pslots = (size_t)p.pgrid * 2 * ba_slot_floats(16 * p.pgroups) * 4;
-    p.row_bytes = (size_t)n * hq * 66 * 4;
-    take(kBaHeadBytes);
-    take(p.pitems * sizeof(BaItem));
-    take((size_t)n_groups * 4);
-    take(p.pslots);
-    take(p.row_bytes);
-    take(p.row_bytes);
-  }
-  p.total = at;
   return p;
 }
 
-void ba_run(int vbits, const BaArgs& a, bool sub, bool prec, bool rows, int groups, unsigned grid, hipStream_t st) {
-  if (vbits == 2) ba_launch<2>(a, sub, prec, rows, groups, grid, st);
-  else if (vbits == 3) ba_launch<3>(a, sub, prec, rows, groups, grid, st);
-  else ba_launch<4>(a, sub, prec, rows, groups, grid, st);
+// Places the workspace's parts from `at` on (null: only counts); the bytes taken.
+size_t ba_place(const BaPlan& p, int64_t n, int hq, char* at, BaArgs* a) {
+  size_t used = 0;
+  auto take = [&](size_t bytes) {
+    char* here = at ? at + used : nullptr;
+    used += align_up(bytes, 256);
+    return here;
+  };
+  const size_t rows = (size_t)n * hq;
+  BaArgs b{};
+  b.tokens = reinterpret_cast<BaToken*>(take(n * sizeof(BaToken)));
+  b.qscale_inv = reinterpret_cast<float*>(take(rows * 4));
+  b.qhi = reinterpret_cast<_Float16*>(take(rows * 128));
+  if (p.prec) b.qlo = reinterpret_cast<_Float16*>(take(rows * 128));
+  for (int l = 0; l < 2; ++l) {
+    if (p.grid[l] == 0) continue;
+    BaLine& ln = b.line[l];
+    ln.waves = (int)p.grid[l] * kBaWaves;
+    ln.rows = p.rw[l] * p.groups[l];
+    ln.max_items = (int)p.items[l];
+    ln.head = reinterpret_cast<BaHead*>(take(sizeof(BaHead)));
+    ln.items = reinterpret_cast<BaItem*>(take(p.items[l] * sizeof(BaItem)));
+    ln.seg_item = reinterpret_cast<int32_t*>(take((p.segs[l] + 1) * 4));
+    ln.work = reinterpret_cast<int32_t*>(take((size_t)ln.waves * 4));
+    ln.slots = reinterpret_cast<float*>(take((size_t)ln.waves * 2 * ba_slot_floats(ln.rows) * 4));
+    ln.row_sums = reinterpret_cast<float*>(take(rows * 256));
+    ln.row_stats = reinterpret_cast<float*>(take(rows * 8));
+  }
+  if (a) {
+    a->tokens = b.tokens; a->qscale_inv = b.qscale_inv; a->qhi = b.qhi; a->qlo = b.qlo;
+    a->line[0] = b.line[0]; a->line[1] = b.line[1];
+  }
+  return used;
+}
+
+void ba_run(int vbits, const BaArgs& a, int l, bool sub, const BaPlan& p, hipStream_t st) {
+  if (vbits == 2) ba_launch<2>(a, l, sub, p.prec, p.rw[l], p.groups[l], p.grid[l], st);
+  else if (vbits == 3) ba_launch<3>(a, l, sub, p.prec, p.rw[l], p.groups[l], p.grid[l], st);
+  else ba_launch<4>(a, l, sub, p.prec, p.rw[l], p.groups[l], p.grid[l], st);
 }
 
 }  // namespace
@@ -220,7 +480,7 @@ extern "C" {
 size_t tq_attention_batch_workspace_bytes(tq_dtype q_dtype, int32_t n_tokens, int32_t hq, int32_t hkv,
                                           int32_t n_seqs, int32_t n_groups, int64_t capacity) {
   if (n_tokens <= 0 || hkv < 1 || hq < hkv || hq % hkv || n_seqs < 0 || n_groups < 0 || capacity < 0) return 0;
-  return ba_plan(q_dtype, n_tokens, hq, hkv, n_seqs, n_groups, capacity).total;
+  return ba_place(ba_plan(q_dtype, n_tokens, hq, hkv, n_seqs, n_groups, capacity), n_tokens, hq, nullptr, nullptr);
 }
 
 int tq_attention_batch_paged_dl(const void* q, tq_dtype q_dtype, int32_t n_tokens, int64_t q_stride, int32_t hq,
@@ -244,6 +504,8 @@ int tq_attention_batch_paged_dl(const void* q, tq_dtype q_dtype, int32_t n_token
   TQ_REQUIRE(block_size >= 16 && (1 << bsl) == block_size,
              "decode-layout pools need a power-of-two block_size >= 16, got %d", block_size);
   TQ_REQUIRE(n_tokens >= 0 && n_seqs >= 0 && n_groups >= 0 && max_blocks >= 0 && num_blocks >= 0, "bad sizes");
+  TQ_REQUIRE(n_seqs < kBaMaxSegs && n_groups <= kBaMaxSegs, "a call takes at most %d sequences and %d groups, got %d and %d",
+             kBaMaxSegs - 1, kBaMaxSegs, n_seqs, n_groups);
   TQ_REQUIRE(num_blocks <= (int64_t)UINT_MAX, "too many blocks");
   TQ_REQUIRE(table_stride >= max_blocks, "table rows of %d entries overlap at a stride of %lld", max_blocks,
              (long long)table_stride);
@@ -273,11 +535,12 @@ int tq_attention_batch_paged_dl(const void* q, tq_dtype q_dtype, int32_t n_token
   const size_t esz = dtype_size(q_dtype);
   TQ_REQUIRE(q_stride * esz % 16 == 0 && out_stride * esz % 16 == 0, "token strides must be multiples of 16 bytes");
   const BaPlan p = ba_plan(q_dtype, n_tokens, hq, hkv, n_seqs, n_groups, cap);
-  TQ_REQUIRE(p.items * hkv * (p.groups) <= INT_MAX && p.pitems * hkv * 3 <= INT_MAX, "too many query rows in one call");
-  TQ_REQUIRE(p.total == 0 || (workspace && workspace_bytes >= p.total), "workspace too small: need %zu bytes", p.total);
-  TQ_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15u) == 0, "workspace must be 16-byte aligned");
-
+  TQ_REQUIRE(p.items[0] <= INT_MAX && p.items[1] <= INT_MAX && (int64_t)n_tokens * hq <= (int64_t)INT_MAX * 16,
+             "too many query rows in one call");
   BaArgs a{};
+  const size_t need = ba_place(p, n_tokens, hq, static_cast<char*>(workspace), &a);
+  TQ_REQUIRE(workspace && workspace_bytes >= need, "workspace too small: need %zu bytes", need);
+  TQ_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15u) == 0, "workspace must be 16-byte aligned");
   a.q = q; a.q_stride = q_stride; a.q_dt = (int)q_dtype;
   a.n_tokens = n_tokens; a.hq = hq; a.hkv = hkv; a.G = hq / hkv; a.B = n_seqs;
   a.query_start = query_start_loc; a.seq_lens = seq_lens;
@@ -295,45 +558,17 @@ int tq_attention_batch_paged_dl(const void* q, tq_dtype q_dtype, int32_t n_token
   a.slopes = v.alibi_slopes; a.window = v.window; a.prefix_lens = v.prefix_lens; a.token_starts = v.token_starts;
   a.out = out; a.out_stride = out_stride; a.lse = lse; a.zero_tail = zero_tail;
   hipStream_t st = as_stream(stream);
-  char* at = static_cast<char*>(workspace);
-  auto take = [&](size_t bytes) {
-    char* here = at;
-    at += align_up(bytes, 256);
-    return here;
-  };
-  if (p.rows) {
-    ba_run(vbits, a, bsl < 6, p.prec, true, p.groups, p.grid, st);
-    TQ_LAUNCH_CHECK("batch_attn_kernel");
-    return TQ_OK;
-  }
-  a.head = reinterpret_cast<BaHead*>(take(kBaHeadBytes));
-  a.items = reinterpret_cast<BaItem*>(take(p.items * sizeof(BaItem)));
-  a.max_items = (int)p.items;
-  a.slots = reinterpret_cast<float*>(take(p.slots));
-  BaPrefix pre{};
-  if (n_groups > 0) {
-    BaArgs b = a;
-    b.over_groups = 1;
-    b.head = reinterpret_cast<BaHead*>(take(kBaHeadBytes));
-    b.items = reinterpret_cast<BaItem*>(take(p.pitems * sizeof(BaItem)));
-    b.max_items = (int)p.pitems;
-    b.seg_item = reinterpret_cast<int32_t*>(take((size_t)n_groups * 4));
-    b.slots = reinterpret_cast<float*>(take(p.pslots));
-    float* mine = reinterpret_cast<float*>(take(p.row_bytes));
-    float* theirs = reinterpret_cast<float*>(take(p.row_bytes));
-    a.row_sums = mine;
-    a.row_stats = mine + (size_t)n_tokens * hq * 64;
-    b.row_sums = theirs;
-    b.row_stats = theirs + (size_t)n_tokens * hq * 64;
-    pre = BaPrefix{b.slots, b.head, b.items, b.seg_item, b.row_sums, b.row_stats, b.max_items, 16 * p.pgroups};
-    ba_run(vbits, b, bsl < 6, p.prec, false, p.pgroups, p.pgrid, st);
+  const int lines = n_groups > 0 ? 2 : 1;
+  const int64_t qrows = (int64_t)n_tokens * hq;
+  hipLaunchKernelGGL(batch_prep_kernel, dim3((unsigned)(lines + (qrows + 16 * kPrepWaves - 1) / (16 * kPrepWaves))),
+                     dim3(kPrepThreads), 0, st, a, lines, p.prec ? 1 : 0);
+  TQ_LAUNCH_CHECK("batch_prep_kernel");
+  for (int l = lines - 1; l >= 0; --l) {
+    ba_run(vbits, a, l, bsl < 6, p, st);
     TQ_LAUNCH_CHECK("batch_attn_kernel");
   }
-  ba_run(vbits, a, bsl < 6, p.prec, false, p.groups, p.grid, st);
-  TQ_LAUNCH_CHECK("batch_attn_kernel");
-  hipLaunchKernelGGL(batch_combine_kernel, dim3((unsigned)(p.items * hkv * p.groups)), dim3(256), 0, st, a, pre,
-                     16 * p.groups, n_groups > 0 ? 1 : 0);
-  TQ_LAUNCH_CHECK("batch_combine_kernel");
+  hipLaunchKernelGGL(batch_join_kernel, dim3((unsigned)((qrows + 15) / 16)), dim3(64 * kJoinWaves), 0, st, a);
+  TQ_LAUNCH_CHECK("batch_join_kernel");
   return TQ_OK;
 }
 

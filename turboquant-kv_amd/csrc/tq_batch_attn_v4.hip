@@ -2,5 +2,5 @@
 #include "tq_batch_attn_kernel.h"
 
 namespace tq {
-template void ba_launch<4>(const BaArgs&, bool, bool, bool, int, unsigned, hipStream_t);
+template void ba_launch<4>(const BaArgs&, int, bool, bool, int, int, unsigned, hipStream_t);
 }  // namespace tq
