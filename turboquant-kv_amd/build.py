@@ -28,7 +28,8 @@ HIP_LIB = os.path.join(LIBDIR, "libturboquant_hip.so")
 TORCH_LIB = os.path.join(LIBDIR, "libturboquant_torch.so")
 
 HIP_SOURCES = ["tq_quantize.hip", "tq_dequant.hip", "tq_append.hip", "tq_scan.hip", "tq_decode.hip", "tq_paged.hip", "tq_prefill.hip",
-               "tq_batch.hip", "tq_batch_attn.hip", "tq_batch_attn_v2.hip", "tq_batch_attn_v3.hip", "tq_batch_attn_v4.hip",
+               "tq_batch.hip", "tq_batch_attn.hip", "tq_batch_attn_2t.hip", "tq_batch_attn_2s.hip",
+               "tq_batch_attn_3t.hip", "tq_batch_attn_3s.hip", "tq_batch_attn_4t.hip", "tq_batch_attn_4s.hip",
                "tq_core_tables.hip", "tq_entropy.hip"]
 # host C++ of the torch.ops library: the HIP-device ops and the CPU-tensor kernels of the
 # reference schemas

@@ -47,8 +47,10 @@
 
 namespace tq {
 
-constexpr int kBaWaves = 8;
-constexpr int kBaThreads = 64 * kBaWaves;
+// Waves of a workgroup (one per CU: the tables fill its LDS).  Single tokens of fp32 / fp16
+// queries: 12 (168 registers a wave) instead of 8 hide more of the three products' latency: 48
+// sequences of up to 32k tokens, 4-bit values, 128 -> 117 us; bf16: 89 and 91 us.
+constexpr int ba_waves(bool prec, int rw, int groups) { return prec && groups == 1 && rw < 16 ? 12 : 8; }
 constexpr int kBaMaxSegs = 8191;  // sequences or groups of a call: the preparing kernel's LDS
 constexpr int kBaOver = 3;        // an (item, head)'s cost besides its tiles, in tiles
 // Row groups of a wave where rows abound: with hi + lo parts two fit the registers.
@@ -69,12 +71,19 @@ struct BaItem {
   int32_t table;      // row of block_tables
   int32_t lo, hi;     // positions this line covers
 };
+// An entry of the tables: byte i's key centroids (c[i / 16], c[i % 16]) and value centroids as
+// fp16 hi and lo parts, scaled by powers of two into [0.5, 1).
+struct BaEntry {
+  uint32_t khi, klo, vhi[2], vlo[2];
+  float vsc_inv;  // the values' scale undone
+  uint32_t pad;
+};
 struct BaLine {
   BaHead* head;
   BaItem* items;
   int32_t max_items;   // entries of `items`
   int32_t* seg_item;   // [segments + 1]: first item of each
-  int32_t* work;       // [waves]: item that the wave's piece begins in, or -1
+  int32_t* work;       // [waves]: the item that the wave's piece begins in; -1: behind the line's end
   int32_t waves;
   int32_t rows;        // R
   float* slots;        // [waves][2][ba_slot_floats(R)]
@@ -122,7 +131,8 @@ struct BaArgs {
   // made by the preparing kernel
   _Float16* qhi;               // [n_tokens * hq][64] rotated queries over a power of two: hi,
   _Float16* qlo;               // and lo parts (fp32 / fp16 queries)
-  float* qscale_inv;           // [n_tokens * hq] that power of two
+  float* qscale_inv;           // [n_tokens * hq] what undoes it and the key centroids' scale
+  BaEntry* entries;            // [256]
   BaToken* tokens;             // [n_tokens]
   BaLine line[2];              // sequences, groups
 };
@@ -132,12 +142,15 @@ typedef _Float16 ba_v8h __attribute__((ext_vector_type(8)));
 typedef uint32_t ba_u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t ba_u32x2 __attribute__((ext_vector_type(2)));
 
-// Launches the main kernel of value width VB over line `l` (rw: 4, 8 or 16 rows a group).
-template <int VB>
-void ba_launch(const BaArgs& a, int l, bool sub, bool prec, int rw, int groups, unsigned grid, hipStream_t st);
-extern template void ba_launch<2>(const BaArgs&, int, bool, bool, int, int, unsigned, hipStream_t);
-extern template void ba_launch<3>(const BaArgs&, int, bool, bool, int, int, unsigned, hipStream_t);
-extern template void ba_launch<4>(const BaArgs&, int, bool, bool, int, int, unsigned, hipStream_t);
+// Launches the main kernel of value width VB over line `l` (rw: 4, 8 or 16 rows a group of
+// columns; SUB: pools of 16-token value sub-blocks; wide: pools of 4 GB and more).
+template <int VB, bool SUB>
+void ba_launch(const BaArgs& a, int l, bool wide, bool prec, int rw, int groups, unsigned grid, hipStream_t st);
+#define BA_LAUNCH(VB, SUB) \
+  template void ba_launch<VB, SUB>(const BaArgs&, int, bool, bool, int, int, unsigned, hipStream_t);
+extern BA_LAUNCH(2, false) extern BA_LAUNCH(2, true)
+extern BA_LAUNCH(3, false) extern BA_LAUNCH(3, true)
+extern BA_LAUNCH(4, false) extern BA_LAUNCH(4, true)
 
 __device__ __forceinline__ int ba_qs(const BaArgs& a, int b) {
   return max(0, min(a.query_start[b], a.n_tokens));
@@ -153,6 +166,11 @@ __device__ __forceinline__ int ba_last(int n, int v, F key) {
     else hi = mid;
   }
   return lo;
+}
+
+// a / b for 0 <= a, 0 < b: places rarely need 64 bits, whose division takes ten times as long.
+__device__ __forceinline__ int64_t ba_div(int64_t a, int64_t b) {
+  return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
 }
 
 // Tiles of an (item, head) before place `place` of it.

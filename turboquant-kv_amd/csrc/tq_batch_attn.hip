@@ -85,10 +85,15 @@ __device__ __forceinline__ void ba_lay_out(const BaArgs& a, int32_t* base_s, int
   const int nseg = L == 1 ? a.n_groups : a.B;
   // first items of the segments
   int64_t run = 0;
+  BaSeg mine{};  // of segment tid, for the common step of one item per segment
   for (int s0 = 0; s0 < nseg; s0 += kPrepThreads) {
     const int s = s0 + tid;
     int64_t n = 0, all;
-    if (s < nseg) n = ((int64_t)ba_segment<L>(a, s).ntok * a.G + R - 1) / R;
+    if (s < nseg) {
+      const BaSeg x = ba_segment<L>(a, s);
+      n = ba_div((int64_t)x.ntok * a.G + R - 1, R);
+      if (s0 == 0) mine = x;
+    }
     const int64_t at = prep_scan(n, part, &all);
     if (s < nseg) base_s[s] = ln.seg_item[s] = (int)min<int64_t>(run + at, INT_MAX);
     run += all;
@@ -103,8 +108,9 @@ __device__ __forceinline__ void ba_lay_out(const BaArgs& a, int32_t* base_s, int
     int64_t cost = 0, all;
     BaItem it{};
     if (i < n_items) {
-      const int s = ba_last(nseg, i, [&](int k) { return base_s[k]; });
-      const BaSeg x = ba_segment<L>(a, s);
+      const bool own = i < kPrepThreads && i < nseg && base_s[i] == i && base_s[i + 1] == i + 1;
+      const int s = own ? i : ba_last(nseg, i, [&](int k) { return base_s[k]; });
+      const BaSeg x = own ? mine : ba_segment<L>(a, s);
       const int64_t row0 = (int64_t)(i - base_s[s]) * R;
       it.tok0 = x.tok0;
       it.row0 = (int)row0;
@@ -116,7 +122,7 @@ __device__ __forceinline__ void ba_lay_out(const BaArgs& a, int32_t* base_s, int
       // their own rows' starts leave out.
       int64_t lo = x.lo, hi = x.hi;
       if (L == 0) {
-        const int i0t = (int)(row0 / a.G), i1t = min(x.ntok - 1, (int)((row0 + R - 1) / a.G));
+        const int i0t = (int)ba_div(row0, a.G), i1t = min(x.ntok - 1, (int)ba_div(row0 + R - 1, a.G));
         hi = min<int64_t>(hi, max<int64_t>((int64_t)x.past + i1t + 1, x.prefix));
         if (a.window > 0) lo = max<int64_t>(lo, (int64_t)x.past + i0t + 1 - a.window);
         if (a.token_starts && x.ntok == 1 && hi > 0) lo = max<int64_t>(lo, a.token_starts[x.tok0]);
@@ -134,9 +140,20 @@ __device__ __forceinline__ void ba_lay_out(const BaArgs& a, int32_t* base_s, int
     place += all;
   }
   // Equal pieces, of a few tiles at least.
-  const int64_t chunk = max<int64_t>(kBaOver + 1, (place + ln.waves - 1) / ln.waves);
+  const int64_t chunk = max<int64_t>(kBaOver + 1, ba_div(place + ln.waves - 1, ln.waves));
   if (tid == 0) *ln.head = BaHead{chunk, place, n_items, 0};
-  // the item that each wave's piece begins in
+  // The item that each wave's piece begins in: a wave per item fills its waves' entries, or,
+  // where items abound, each entry searches for its own.
+  if (n_items <= 8 * kPrepWaves) {
+    __syncthreads();
+    for (int i = tid >> 6; i < n_items; i += kPrepWaves) {
+      const int64_t from = start_s[i], to = i + 1 < n_items ? start_s[i + 1] : place;
+      const int w1 = (int)ba_div(to + chunk - 1, chunk);
+      for (int w = (int)ba_div(from + chunk - 1, chunk) + (tid & 63); w < w1; w += 64) ln.work[w] = i;
+    }
+    for (int w = (int)ba_div(place + chunk - 1, chunk) + tid; w < ln.waves; w += kPrepThreads) ln.work[w] = -1;
+    return;
+  }
   auto start_of = [&](int i) { return n_items <= kPrepStarts ? start_s[i] : ln.items[i].start; };
   __syncthreads();
   for (int w = tid; w < ln.waves; w += kPrepThreads) {
@@ -151,10 +168,40 @@ __device__ __forceinline__ void ba_lay_out(const BaArgs& a, int32_t* base_s, int
   }
 }
 
+__device__ __forceinline__ uint32_t ba_pack(_Float16 lo, _Float16 hi) {
+  typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, (h2_t){lo, hi});
+}
+
+// The exponent e of amax = m 2^e, m in [0.5, 1) (0 for 0, inf or NaN).
+__device__ __forceinline__ int ba_exponent(float amax) {
+  int e = 0;
+  if (amax > 0.f && amax < INFINITY) frexpf(amax, &e);
+  return e;
+}
+
+// Entry `e` of the tables, for centroids of exponents ke and ve.
+__device__ __forceinline__ BaEntry ba_entry(const BaArgs& a, int vbits, int e, int ke, int ve) {
+  BaEntry x{};
+  const float ksc = ldexpf(1.f, -ke), vsc = ldexpf(1.f, -ve);
+  auto split = [](float u, float v, uint32_t& hi, uint32_t& lo) {
+    const _Float16 hu = (_Float16)u, hv = (_Float16)v;
+    hi = ba_pack(hu, hv);
+    lo = ba_pack((_Float16)(u - (float)hu), (_Float16)(v - (float)hv));
+  };
+  split(a.kcen[e >> 4] * ksc, a.kcen[e & 15] * ksc, x.khi, x.klo);
+  const int mask = (1 << vbits) - 1;
+  // a byte's four tokens (2 bits), or a pair (3 bits: its top two bits belong to another dim)
+  split(a.vcen[e & mask] * vsc, a.vcen[(e >> vbits) & mask] * vsc, x.vhi[0], x.vlo[0]);
+  if (vbits == 2) split(a.vcen[(e >> 4) & 3] * vsc, a.vcen[(e >> 6) & 3] * vsc, x.vhi[1], x.vlo[1]);
+  x.vsc_inv = ldexpf(1.f, ve);
+  return x;
+}
+
 // Workgroups 0 .. n_lines - 1 lay the lines out; the others rotate 16 rows (a token's head
 // each) a wave: Qrot = (q * qscale) R_k^T by v_mfma_f32_16x16x4f32, scaled by a power of two
 // into [0.5, 1) and split into fp16 hi (and lo) parts, and find their tokens' positions.
-__global__ __launch_bounds__(kPrepThreads) void batch_prep_kernel(BaArgs a, int n_lines, int prec) {
+__global__ __launch_bounds__(kPrepThreads) void batch_prep_kernel(BaArgs a, int n_lines, int prec, int vbits) {
 #pragma clang fp contract(off)
   __shared__ int32_t base_s[kBaMaxSegs + 2];
   __shared__ int64_t start_s[kPrepStarts];
@@ -189,13 +236,19 @@ __global__ __launch_bounds__(kPrepThreads) void batch_prep_kernel(BaArgs a, int 
     }
     a.tokens[t] = x;
   }
+  // ---- the centroids' scales; the tables' entries (once)
+  const int ke = ba_exponent(wave_max(lane < 16 ? fabsf(a.kcen[lane]) : 0.f));
+  if (blk == 0 && tid < 256) {
+    const int ve = ba_exponent(wave_max(lane < (1 << vbits) ? fabsf(a.vcen[lane]) : 0.f));
+    a.entries[tid] = ba_entry(a, vbits, tid, ke, ve);
+  }
   // ---- rows.  MFMA mb, k-step s: lane (c, g) supplies A[c][g] = R_k[16 (c / 4) + 4 mb + c % 4][16 g + s]
   // and B[g][c] = q_c[16 g + s]; register r of lane (c, g) gets Qrot_c[16 g + 4 mb + r]: a lane
   // ends with dims 16 g .. 16 g + 15, the order in which its key bytes come.
   const int64_t r0 = (blk * kPrepWaves + wave) * 16;
   if (r0 >= n_rows) return;
   const int64_t row = min(r0 + c, n_rows - 1);
-  const int64_t qo = row / a.hq * a.q_stride + row % a.hq * 64 + 16 * g;
+  const int64_t qt = ba_div(row, a.hq), qo = qt * a.q_stride + (row - qt * a.hq) * 64 + 16 * g;
   float qv[16];
   if (a.q_dt == TQ_F32) {
     const ba_v4f* src = reinterpret_cast<const ba_v4f*>(static_cast<const float*>(a.q) + qo);
@@ -237,8 +290,7 @@ __global__ __launch_bounds__(kPrepThreads) void batch_prep_kernel(BaArgs a, int 
     for (int r = 0; r < 4; ++r) qm = fmaxf(qm, fabsf(d[mb][r]));
   qm = fmaxf(qm, __shfl_xor(qm, 16, 64));
   qm = fmaxf(qm, __shfl_xor(qm, 32, 64));
-  int e = 0;
-  if (qm > 0.f && qm < INFINITY) frexpf(qm, &e);
+  const int e = ba_exponent(qm);
   const float qsc = ldexpf(1.f, -e);
   ba_v8h hi[2], lo[2];
 #pragma unroll
@@ -255,7 +307,7 @@ __global__ __launch_bounds__(kPrepThreads) void batch_prep_kernel(BaArgs a, int 
     *reinterpret_cast<ba_v8h*>(a.qhi + row * 64 + 16 * g + 8 * s) = hi[s];
     if (prec) *reinterpret_cast<ba_v8h*>(a.qlo + row * 64 + 16 * g + 8 * s) = lo[s];
   }
-  if (g == 0) a.qscale_inv[row] = ldexpf(1.f, e);
+  if (g == 0) a.qscale_inv[row] = ldexpf(1.f, e + ke);
 }
 
 // ------------------------------------------------------------------------------- joining
@@ -272,14 +324,14 @@ __device__ __forceinline__ BaFrom ba_from(const BaArgs& a, const BaLine& ln, int
   BaFrom f{};
   const int n_items = ln.head->n_items;
   if (n_items <= 0 || seg_row < 0) return f;
-  const BaItem it = ln.items[max(0, min(ln.seg_item[seg] + (int)(seg_row / ln.rows), n_items - 1))];
+  const BaItem it = ln.items[max(0, min(ln.seg_item[seg] + (int)ba_div(seg_row, ln.rows), n_items - 1))];
   const int64_t chunk = ln.head->chunk;
   const int cost = it.nt + kBaOver;
   const int64_t start = it.start + (int64_t)h * cost;
-  f.row = (int)(seg_row % ln.rows);
+  f.row = (int)(seg_row - ba_div(seg_row, ln.rows) * ln.rows);
   // the waves that the first and the last tile fall to
-  f.w0 = (start + kBaOver) / chunk;
-  const int64_t w1 = (start + cost - 1) / chunk;
+  f.w0 = ba_div(start + kBaOver, chunk);
+  const int64_t w1 = ba_div(start + cost - 1, chunk);
   f.by_row = it.nt == 0 || f.w0 == w1;
   f.count = f.by_row ? 1 : (int)(w1 - f.w0) + 1;
   return f;
@@ -300,7 +352,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void batch_join_kernel(BaArgs a) {
   const int c = lane & 15, g = lane >> 4;
   const int64_t n_rows = (int64_t)a.n_tokens * a.hq, r0 = (int64_t)blockIdx.x * 16;
   const int64_t rowid = min(r0 + c, n_rows - 1);
-  const int tok = (int)(rowid / a.hq), qh = (int)(rowid - (int64_t)tok * a.hq);
+  const int tok = (int)ba_div(rowid, a.hq), qh = (int)(rowid - (int64_t)tok * a.hq);
   const int h = qh / a.G, gq = qh - h * a.G;
   // R_v's entries of this wave's dims, wanted last
   float rv[16];
@@ -439,6 +491,7 @@ size_t ba_place(const BaPlan& p, int64_t n, int hq, char* at, BaArgs* a) {
   };
   const size_t rows = (size_t)n * hq;
   BaArgs b{};
+  b.entries = reinterpret_cast<BaEntry*>(take(256 * sizeof(BaEntry)));
   b.tokens = reinterpret_cast<BaToken*>(take(n * sizeof(BaToken)));
   b.qscale_inv = reinterpret_cast<float*>(take(rows * 4));
   b.qhi = reinterpret_cast<_Float16*>(take(rows * 128));
@@ -446,7 +499,7 @@ size_t ba_place(const BaPlan& p, int64_t n, int hq, char* at, BaArgs* a) {
   for (int l = 0; l < 2; ++l) {
     if (p.grid[l] == 0) continue;
     BaLine& ln = b.line[l];
-    ln.waves = (int)p.grid[l] * kBaWaves;
+    ln.waves = (int)p.grid[l] * ba_waves(p.prec, p.rw[l], p.groups[l]);
     ln.rows = p.rw[l] * p.groups[l];
     ln.max_items = (int)p.items[l];
     ln.head = reinterpret_cast<BaHead*>(take(sizeof(BaHead)));
@@ -458,16 +511,23 @@ size_t ba_place(const BaPlan& p, int64_t n, int hq, char* at, BaArgs* a) {
     ln.row_stats = reinterpret_cast<float*>(take(rows * 8));
   }
   if (a) {
-    a->tokens = b.tokens; a->qscale_inv = b.qscale_inv; a->qhi = b.qhi; a->qlo = b.qlo;
+    a->entries = b.entries; a->tokens = b.tokens; a->qscale_inv = b.qscale_inv; a->qhi = b.qhi; a->qlo = b.qlo;
     a->line[0] = b.line[0]; a->line[1] = b.line[1];
   }
   return used;
 }
 
-void ba_run(int vbits, const BaArgs& a, int l, bool sub, const BaPlan& p, hipStream_t st) {
-  if (vbits == 2) ba_launch<2>(a, l, sub, p.prec, p.rw[l], p.groups[l], p.grid[l], st);
-  else if (vbits == 3) ba_launch<3>(a, l, sub, p.prec, p.rw[l], p.groups[l], p.grid[l], st);
-  else ba_launch<4>(a, l, sub, p.prec, p.rw[l], p.groups[l], p.grid[l], st);
+template <int VB>
+void ba_run_bits(const BaArgs& a, int l, const BaPlan& p, hipStream_t st) {
+  const bool wide = (uint64_t)a.num_blocks * a.hkv << a.bs_log2 > 0xFFFFFFFFu / 32;  // key bytes past 32 bits
+  if (a.bs_log2 < 6) ba_launch<VB, true>(a, l, wide, p.prec, p.rw[l], p.groups[l], p.grid[l], st);
+  else ba_launch<VB, false>(a, l, wide, p.prec, p.rw[l], p.groups[l], p.grid[l], st);
+}
+
+void ba_run(int vbits, const BaArgs& a, int l, const BaPlan& p, hipStream_t st) {
+  if (vbits == 2) ba_run_bits<2>(a, l, p, st);
+  else if (vbits == 3) ba_run_bits<3>(a, l, p, st);
+  else ba_run_bits<4>(a, l, p, st);
 }
 
 }  // namespace
@@ -561,10 +621,10 @@ int tq_attention_batch_paged_dl(const void* q, tq_dtype q_dtype, int32_t n_token
   const int lines = n_groups > 0 ? 2 : 1;
   const int64_t qrows = (int64_t)n_tokens * hq;
   hipLaunchKernelGGL(batch_prep_kernel, dim3((unsigned)(lines + (qrows + 16 * kPrepWaves - 1) / (16 * kPrepWaves))),
-                     dim3(kPrepThreads), 0, st, a, lines, p.prec ? 1 : 0);
+                     dim3(kPrepThreads), 0, st, a, lines, p.prec ? 1 : 0, vbits);
   TQ_LAUNCH_CHECK("batch_prep_kernel");
   for (int l = lines - 1; l >= 0; --l) {
-    ba_run(vbits, a, l, bsl < 6, p, st);
+    ba_run(vbits, a, l, p, st);
     TQ_LAUNCH_CHECK("batch_attn_kernel");
   }
   hipLaunchKernelGGL(batch_join_kernel, dim3((unsigned)((qrows + 15) / 16)), dim3(64 * kJoinWaves), 0, st, a);

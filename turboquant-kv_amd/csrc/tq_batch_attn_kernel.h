@@ -8,24 +8,11 @@ namespace {
 
 // LDS: key table, value table, each wave's norms of a tile.
 constexpr int kBaVTab = 65536;
-constexpr int kBaNorms = 131072;  // [8 waves][2][64] floats
-constexpr int kBaLds = kBaNorms + kBaWaves * 512;
+constexpr int kBaNorms = 131072;  // [waves][2][64] floats
 
 __device__ __forceinline__ ba_v8h ba_h8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   ba_u32x4 t = {a, b, c, d};
   return __builtin_bit_cast(ba_v8h, t);
-}
-
-__device__ __forceinline__ uint32_t ba_pack(_Float16 lo, _Float16 hi) {
-  typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
-  return __builtin_bit_cast(uint32_t, (h2_t){lo, hi});
-}
-
-// 2^-e with amax = m 2^e, m in [0.5, 1) (1 for 0, inf or NaN)
-__device__ __forceinline__ float ba_pow2_scale(float amax) {
-  int e = 0;
-  if (amax > 0.f && amax < INFINITY) frexpf(amax, &e);
-  return ldexpf(1.f, -e);
 }
 
 // cap2 tanh(y / cap2).  tanh z = 1 - 2 / (1 + e^(2 z)), exact at both ends (the exponential
@@ -58,20 +45,41 @@ __device__ __forceinline__ int ba_wave_min(int v) {
 __device__ __forceinline__ int ba_wave_max(int v) { return -ba_wave_min(-v); }
 
 
-// The larger of x over the lanes c, c + 16, c + 32, c + 48.
-__device__ __forceinline__ float ba_max4(float x) {
-  x = fmaxf(x, __shfl_xor(x, 16, 64));
-  return fmaxf(x, __shfl_xor(x, 32, 64));
+// Loads through a raw buffer resource: a lane's 32-bit offset plus a scalar one, no vector
+// address arithmetic.
+template <typename T>
+__device__ __forceinline__ T ba_load(__amdgpu_buffer_rsrc_t rs, uint32_t lane_off, uint32_t off) {
+  if constexpr (sizeof(T) == 4) return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(rs, lane_off, off, 0));
+  else if constexpr (sizeof(T) == 8) return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b64(rs, lane_off, off, 0));
+  else return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b128(rs, lane_off, off, 0));
 }
 
-// RW rows of 16 columns (16 / RW copies share a tile's tokens), NGR groups of columns.
-template <int VB, bool SUB, bool PREC, int RW, int NGR>
-__global__ __launch_bounds__(kBaThreads, 2) void batch_attn_kernel(BaArgs a, BaLine ln) {
+// The larger of two numbers in one instruction (fmaxf first quiets operands it cannot see
+// through); NaN yields the other one.
+__device__ __forceinline__ float ba_max(float a, float b) {
+  float r;
+  asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
+}
+
+// The larger of x over the lanes c, c + 16, c + 32, c + 48.
+__device__ __forceinline__ float ba_max4(float x) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = ba_max(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return ba_max(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+// RW rows of 16 columns (16 / RW copies share a tile's tokens), NGR groups of columns.  WIDE: pools
+// of 4 GB and more, whose rows need 64-bit addresses.
+template <int VB, bool SUB, bool PREC, int RW, int NGR, bool WIDE>
+__global__ __launch_bounds__(64 * ba_waves(PREC, RW, NGR), ba_waves(PREC, RW, NGR) / 4) void batch_attn_kernel(BaArgs a, BaLine ln) {
 #pragma clang fp contract(off)
   static_assert(NGR == 1 || RW == 16, "groups of columns hold 16 rows each");
   constexpr int NB = RW / 4;       // 16-token groups whose scores a lane keeps
   constexpr int R = RW * NGR;
-  __shared__ __attribute__((aligned(16))) uint8_t smem[kBaLds];
+  constexpr int WAVES = ba_waves(PREC, RW, NGR);
+  __shared__ __attribute__((aligned(16))) uint8_t smem[kBaNorms + WAVES * 512];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, g = lane >> 4;
@@ -83,117 +91,98 @@ __global__ __launch_bounds__(kBaThreads, 2) void batch_attn_kernel(BaArgs a, BaL
   // pieces spread over the workgroups.
   const unsigned grid = gridDim.x;
   const unsigned blk = grid % 8 == 0 ? (blockIdx.x % 8) * (grid / 8) + blockIdx.x / 8 : blockIdx.x;
-  if (ln.work[blk] < 0) return;  // the workgroup's first piece: there is none behind the line's end
+  if (ln.work[blk] < 0) return;  // the workgroup's first piece: it lies behind the line's end
   const int w = wave * (int)grid + (int)blk;
-  int item = ln.work[w];
-  const int64_t chunk = ln.head->chunk, total = ln.head->total;
+  int item = __builtin_amdgcn_readfirstlane(ln.work[w]);
+  BaItem it = ln.items[max(item, 0)];
+  auto uniform64 = [](int64_t x) {
+    return (int64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)x) |
+           (int64_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32;
+  };
+  const int64_t chunk = uniform64(ln.head->chunk), total = uniform64(ln.head->total);
 
-  // ---- centroid tables scaled by powers of two into [0.5, 1): fp16 hi (and lo) parts
-  float ksc, vsc;
+  // ---- the tables, from the entries that the preparing kernel made
   {
-    float* sc = reinterpret_cast<float*>(smem + kBaNorms);
-    if (wave == 0) {
-      const float km = wave_max(lane < 16 ? fabsf(a.kcen[lane]) : 0.f);
-      const float vm = wave_max(lane < (1 << VB) ? fabsf(a.vcen[lane]) : 0.f);
-      if (lane == 0) {
-        sc[0] = ba_pow2_scale(km);
-        sc[1] = ba_pow2_scale(vm);
-      }
-    }
-    __syncthreads();
-    ksc = sc[0];
-    vsc = sc[1];
-    const int e = tid & 255, half = tid >> 8;  // entry, 128-byte half: the hi parts (PREC: the lo parts in half 1)
-    ba_u32x4 kq, vq;
-    {
-      const float c0 = a.kcen[e >> 4] * ksc, c1 = a.kcen[e & 15] * ksc;
-      const _Float16 h0 = (_Float16)c0, h1 = (_Float16)c1;
-      const uint32_t hi = ba_pack(h0, h1);
-      const uint32_t lo = ba_pack((_Float16)(c0 - (float)h0), (_Float16)(c1 - (float)h1));
-      const uint32_t x = PREC && half ? lo : hi;
-      kq = (ba_u32x4){x, x, x, x};
-    }
-    if constexpr (VB == 2) {  // the centroids of a byte's four tokens
-      _Float16 vh[4], vl[4];
+    const int e = tid & 255;  // threads t, t + 256, .. write entry t's copies in turn, 16 bytes each
+    const BaEntry x = a.entries[e];
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const float v = a.vcen[(e >> (2 * t)) & 3] * vsc;
-        vh[t] = (_Float16)v;
-        vl[t] = (_Float16)(v - (float)vh[t]);
-      }
-      const uint32_t h0 = ba_pack(vh[0], vh[1]), h1 = ba_pack(vh[2], vh[3]);
-      const uint32_t l0 = ba_pack(vl[0], vl[1]), l1 = ba_pack(vl[2], vl[3]);
-      vq = PREC && half ? (ba_u32x4){l0, l1, l0, l1} : (ba_u32x4){h0, h1, h0, h1};
-    } else {  // of a token pair (3 bits: the byte's top two bits belong to another dim)
-      constexpr int mask = (1 << VB) - 1;
-      const float x0 = a.vcen[e & mask] * vsc, x1 = a.vcen[(e >> VB) & mask] * vsc;
-      const _Float16 y0 = (_Float16)x0, y1 = (_Float16)x1;
-      const uint32_t hi = ba_pack(y0, y1);
-      const uint32_t lo = ba_pack((_Float16)(x0 - (float)y0), (_Float16)(x1 - (float)y1));
-      const uint32_t x = PREC && half ? lo : hi;
-      vq = (ba_u32x4){x, x, x, x};
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      // rotated by the entry so that a wave's stores spread over the banks
-      const int o = e * 256 + half * 128 + 16 * ((j + e) & 7);
-      *reinterpret_cast<ba_u32x4*>(smem + o) = kq;
-      *reinterpret_cast<ba_u32x4*>(smem + kBaVTab + o) = vq;
+    for (int k = tid >> 8; k < 16; k += WAVES / 4) {
+      // rotated by the entry so that a wave's stores spread over the banks; PREC: the lo parts'
+      // copies fill the second 128 bytes
+      const int q = (k + e) & 15;
+      const bool second = PREC && q >= 8;
+      const uint32_t kx = second ? x.klo : x.khi;
+      const uint32_t v0 = second ? x.vlo[0] : x.vhi[0], v1 = VB == 2 ? (second ? x.vlo[1] : x.vhi[1]) : v0;
+      *reinterpret_cast<ba_u32x4*>(smem + e * 256 + 16 * q) = (ba_u32x4){kx, kx, kx, kx};
+      *reinterpret_cast<ba_u32x4*>(smem + kBaVTab + e * 256 + 16 * q) = (ba_u32x4){v0, v1, v0, v1};
     }
     __syncthreads();
   }
+  const float vsc_inv = a.entries[0].vsc_inv;  // a power of two
   // this lane's copy of an entry's hi part (PREC: its lo part is 128 bytes on)
   const uint32_t koff = PREC ? 4u * (lane & 31) : 4u * lane;
-  const uint32_t voff = VB == 2 ? (PREC ? 8u * (lane & 15) : 8u * (lane & 31)) : koff;
+  // (byte 1: the value table's 64 KB, byte 2 of its addresses)
+  const uint32_t voff = (VB == 2 ? (PREC ? 8u * (lane & 15) : 8u * (lane & 31)) : koff) | 0x100u;
+  static_assert(kBaVTab == 0x10000, "value table");
   // address of byte i of w: entry i * 256 + copy
   auto kaddr = [&](uint32_t w, int i) -> uint32_t {
     return __builtin_amdgcn_perm(koff, w, 0x0c0c0004u | ((uint32_t)i << 8));
   };
+  const uint32_t vsel = lane & 1 ? 0x07060302u : 0x05040100u;  // a lane's half of shared words
   auto vaddr = [&](uint32_t w, int i) -> uint32_t {
-    return __builtin_amdgcn_perm(voff, w, 0x0c0c0004u | ((uint32_t)i << 8));
+    return __builtin_amdgcn_perm(voff, w, 0x0c050004u | ((uint32_t)i << 8));
   };
 
 
   if (item < 0) return;
   const int bsl = a.bs_log2;
   float* const snorm = reinterpret_cast<float*>(smem + kBaNorms) + wave * 128;
+  const __amdgpu_buffer_rsrc_t krs = buf_rsrc(a.kpairs, 0xFFFFFFFFu), vrs = buf_rsrc(a.vtiles, 0xFFFFFFFFu);
+  const __amdgpu_buffer_rsrc_t knrs = buf_rsrc(a.knorms, 0xFFFFFFFFu), vnrs = buf_rsrc(a.vnorms, 0xFFFFFFFFu);
   const bool mods = a.cap2 != 0.f || a.slopes != nullptr;
   int64_t pos = (int64_t)w * chunk;
   const int64_t end = min(pos + chunk, total);
 
   while (pos < end) {  // (item, head)s of the piece
-    const BaItem it = ln.items[item];
     const int t0 = __builtin_amdgcn_readfirstlane(it.t0), nt = __builtin_amdgcn_readfirstlane(it.nt);
     const int tok0 = __builtin_amdgcn_readfirstlane(it.tok0), row0 = __builtin_amdgcn_readfirstlane(it.row0);
     const int lastrow = __builtin_amdgcn_readfirstlane(it.nrows) - 1;
     const int table = __builtin_amdgcn_readfirstlane(it.table);
     const int cost = nt + kBaOver;
-    const int h = __builtin_amdgcn_readfirstlane((int)((pos - it.start) / cost));
-    const int off = __builtin_amdgcn_readfirstlane((int)(pos - it.start - (int64_t)h * cost));
+    const int64_t start = uniform64(it.start);
+    const int h = (int)ba_div(pos - start, cost);
+    const int off = (int)(pos - start - (int64_t)h * cost);
     const int n = (int)min<int64_t>(cost - off, end - pos);
     const int ta = (int)ba_tiles(off), tb = (int)ba_tiles(off + n);
     const bool whole = tb - ta == nt && (nt > 0 || off == 0);
     pos += n;
-    if (off + n == cost && h == hkv - 1) ++item;
-    if (!whole && ta == tb) continue;
+    const int it_lo = __builtin_amdgcn_readfirstlane(it.lo), it_hi = __builtin_amdgcn_readfirstlane(it.hi);
+    const bool next = off + n == cost && h == hkv - 1 && pos < end;
+    if (!whole && ta == tb) {
+      if (next) it = ln.items[++item];
+      continue;
+    }
 
+    auto place_of = [&](int j, int& tok, int& qh) {
+      const int row = min(row0 + 16 * j + cr, lastrow), ti = row / G;
+      tok = tok0 + ti;
+      qh = h * G + (row - ti * G);
+    };
     // ---- rows: group j's column c holds row row0 + 16 j + cr (past the end: the last)
-    int tok[NGR], qh[NGR], lo[NGR], hi[NGR], qpos[NGR];
+    int lo[NGR], hi[NGR], qpos[NGR];
     float slope[NGR], kinv[NGR];
     ba_v8h qhi[NGR][2], qlo[PREC ? NGR : 1][2];
 #pragma unroll
     for (int j = 0; j < NGR; ++j) {
-      const int row = min(row0 + 16 * j + cr, lastrow);
-      const int ti = row / G;
-      tok[j] = tok0 + ti;
-      qh[j] = h * G + (row - ti * G);
-      const BaToken t = a.tokens[tok[j]];
-      lo[j] = max(t.lo, it.lo);
-      hi[j] = min(t.hi, it.hi);
+      int tok, qh;
+      place_of(j, tok, qh);
+      const BaToken t = a.tokens[tok];
+      lo[j] = max(t.lo, it_lo);
+      hi[j] = min(t.hi, it_hi);
       qpos[j] = t.pos;
-      const int64_t rowid = (int64_t)tok[j] * a.hq + qh[j];
-      kinv[j] = a.qscale_inv[rowid] / ksc;  // powers of two
-      slope[j] = a.slopes ? a.slopes[qh[j]] * 1.4426950408889634f : 0.f;
+      const int64_t rowid = (int64_t)tok * a.hq + qh;
+      kinv[j] = a.qscale_inv[rowid];
+      slope[j] = a.slopes ? a.slopes[qh] * 1.4426950408889634f : 0.f;
 #pragma unroll
       for (int s = 0; s < 2; ++s) {  // dims 16 g + 8 s ..
         qhi[j][s] = *reinterpret_cast<const ba_v8h*>(a.qhi + rowid * 64 + 16 * g + 8 * s);
@@ -212,10 +201,13 @@ __global__ __launch_bounds__(kBaThreads, 2) void batch_attn_kernel(BaArgs a, BaL
     lo_max = ba_wave_max(lo_max);
     hi_min = ba_wave_min(hi_min);
     hi_max = ba_wave_max(hi_max);
-    // tiles of the piece that some row sees
-    const int k0 = max(t0 + ta, lo_min >> 6);
-    const int k1 = hi_max > lo_min ? min(t0 + tb, (int)(((int64_t)hi_max + 63) >> 6)) : k0;
-    const int nw = max(0, k1 - k0);
+    // tiles of the piece; document starts may leave out some that the line holds
+    int k0 = t0 + ta, nw = tb - ta;
+    if (a.token_starts) {
+      const int k1 = hi_max > lo_min ? min(k0 + nw, (int)(((int64_t)hi_max + 63) >> 6)) : k0;
+      k0 = max(k0, lo_min >> 6);
+      nw = max(0, k1 - k0);
+    }
 
     float m[NGR], l[NGR];
     ba_v4f o[NGR][4];
@@ -228,14 +220,19 @@ __global__ __launch_bounds__(kBaThreads, 2) void batch_attn_kernel(BaArgs a, BaL
       for (int nb = 0; nb < 4; ++nb) o[j][nb] = (ba_v4f){0.f, 0.f, 0.f, 0.f};
     }
 
-    // Block ids of 16 tiles at a time, the next 16 requested while these are used: lane
-    // 4 i + b holds the block of tile i's 16-token group b.
+    // Pool rows of 16 tiles' 16-token groups at a time (lane 4 i + b: tile i's group b), the next
+    // 16 tiles' block ids requested while these are used.
     const int32_t* btab = a.block_tables + (int64_t)table * a.table_stride;
     auto load_ids = [&](int chunk16) -> uint32_t {
       const int i = min(chunk16 * 16 + (lane >> 2), nw - 1);
       const int64_t tb = ((int64_t)(k0 + i) << 6) + 16 * (lane & 3);
       const int bi = (int)min<int64_t>(tb >> bsl, (int64_t)a.max_blocks - 1);
-      return min((uint32_t)btab[bi], a.num_blocks - 1u);
+      return (uint32_t)btab[bi];
+    };
+    using row_t = std::conditional_t<WIDE, uint64_t, uint32_t>;
+    auto pool_row = [&](uint32_t id, int chunk16) -> row_t {
+      const uint32_t tb = ((uint32_t)(k0 + chunk16 * 16 + (lane >> 2)) << 6) + 16u * (lane & 3);
+      return (((row_t)min(id, a.num_blocks - 1u) * (uint32_t)hkv + (uint32_t)h) << bsl) + (tb & ((1u << bsl) - 1u));
     };
     constexpr int NV = VB == 2 ? 4 : (SUB ? 8 : 2 * VB);
     struct Tile {
@@ -243,73 +240,86 @@ __global__ __launch_bounds__(kBaThreads, 2) void batch_attn_kernel(BaArgs a, BaL
       float nk, nv;
       uint32_t vw[NV];
     };
-    uint32_t ids = 0, ids_next = 0;
-    if (nw > 0) {
-      ids_next = load_ids(0);
-    }
+    row_t rows16 = 0;
+    uint32_t ids_next = 0;
+    if (nw > 0) ids_next = load_ids(0);
     // i: the wave's i-th tile, asked for in order (a repeated last one excepted)
     auto load = [&](int i, Tile& t) {
       if ((i & 15) == 0 && i < nw) {
-        ids = ids_next;
+        rows16 = pool_row(ids_next, i >> 4);
         ids_next = load_ids((i >> 4) + 1);
       }
-      const int il = min(i, nw - 1);
-      const int64_t tb0 = (int64_t)(k0 + il) << 6;
-      const int64_t bsm = ((int64_t)1 << bsl) - 1;
-      int64_t base[4];
+      const int from = 4 * (min(i, nw - 1) & 15);
+      auto row_of = [&](int b) -> row_t {  // of 16-token group b
+        row_t r = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)rows16, from + b);
+        if constexpr (WIDE) r |= (row_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(rows16 >> 32), from + b) << 32;
+        return r;
+      };
+      // T at `extra` bytes plus a lane's offset into the bytes of row `r` of a pool
+      auto at = [&](auto tag, const void* pool, __amdgpu_buffer_rsrc_t rs, uint32_t lane_off, row_t r, int bytes, int extra = 0) {
+        using T = decltype(tag);
+        if constexpr (WIDE)
+          return ba_load<T>(buf_rsrc(static_cast<const uint8_t*>(pool) + r * bytes + extra, 0xFFFFFFFFu), lane_off, 0);
+        else
+          return ba_load<T>(rs, lane_off + extra, (uint32_t)r * bytes);
+      };
+      row_t row[4];
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        if (SUB || b == 0) {
-          const uint32_t blk = (uint32_t)__builtin_amdgcn_readlane((int)ids, 4 * (il & 15) + b);
-          base[b] = (((int64_t)blk * hkv + h) << bsl) + ((tb0 + 16 * b) & bsm);
+      for (int b = 0; b < 4; ++b) row[b] = SUB || b == 0 ? row_of(b) : row[0] + 16 * b;
+      if constexpr (SUB) {  // a lane's token: number c of group g
+        const int src = 4 * (from + g);
+        uint32_t lo32 = (uint32_t)__builtin_amdgcn_ds_bpermute(src, (int)(uint32_t)rows16);
+        if constexpr (WIDE) {
+          const row_t r = lo32 | (row_t)(uint32_t)__builtin_amdgcn_ds_bpermute(src, (int)(uint32_t)(rows16 >> 32)) << 32;
+          t.nk = a.knorms[r + (uint32_t)c];
+          t.nv = a.vnorms[r + (uint32_t)c];
         } else {
-          base[b] = base[0] + 16 * b;
+          t.nk = ba_load<float>(knrs, 4u * (lo32 + (uint32_t)c), 0);
+          t.nv = ba_load<float>(vnrs, 4u * (lo32 + (uint32_t)c), 0);
         }
+      } else {
+        t.nk = at(float{}, a.knorms, knrs, 4u * lane, row[0], 4);
+        t.nv = at(float{}, a.vnorms, vnrs, 4u * lane, row[0], 4);
       }
 #pragma unroll
-      for (int b = 0; b < 4; ++b)
-        t.kw[b] = *reinterpret_cast<const ba_u32x2*>(a.kpairs + base[b] * 32 + (c * 32 + 8 * g));
-      {
-        const int64_t nbase = SUB ? (g == 0 ? base[0] : g == 1 ? base[1] : g == 2 ? base[2] : base[3]) + c
-                                  : base[0] + lane;
-        t.nk = a.knorms[nbase];
-        t.nv = a.vnorms[nbase];
-      }
+      for (int b = 0; b < 4; ++b) t.kw[b] = at(ba_u32x2{}, a.kpairs, krs, 32u * c + 8u * g, row[b], 32);
       if constexpr (SUB) {
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-          const uint8_t* sb = a.vtiles + base[b] * (8 * VB);
           if constexpr (VB == 2) {
-            t.vw[b] = *reinterpret_cast<const uint32_t*>(sb + 4 * lane);
+            t.vw[b] = at(uint32_t{}, a.vtiles, vrs, 4u * lane, row[b], 8 * VB);
           } else if constexpr (VB == 4) {
-            const ba_u32x2 w = *reinterpret_cast<const ba_u32x2*>(sb + 8 * lane);
-            t.vw[2 * b] = w.x;
-            t.vw[2 * b + 1] = w.y;
-          } else {
-            t.vw[b] = *reinterpret_cast<const uint32_t*>(sb + 4 * lane);
-            t.vw[4 + b] = *reinterpret_cast<const uint16_t*>(sb + 256 + 2 * lane);
+            const ba_u32x2 x = at(ba_u32x2{}, a.vtiles, vrs, 8u * lane, row[b], 8 * VB);
+            t.vw[2 * b] = x.x;
+            t.vw[2 * b + 1] = x.y;
+          } else {  // the 16-bit share comes with its neighbour's: vsel picks it
+            t.vw[b] = at(uint32_t{}, a.vtiles, vrs, 4u * lane, row[b], 8 * VB);
+            t.vw[4 + b] = at(uint32_t{}, a.vtiles, vrs, 4u * (lane >> 1), row[b], 8 * VB, 256);
           }
         }
       } else {
-        const uint8_t* tb = a.vtiles + base[0] * (8 * VB);
-        const ba_u32x4 v = *reinterpret_cast<const ba_u32x4*>(tb + 16 * lane);
+        const ba_u32x4 v = at(ba_u32x4{}, a.vtiles, vrs, 16u * lane, row[0], 8 * VB);
         t.vw[0] = v.x; t.vw[1] = v.y; t.vw[2] = v.z; t.vw[3] = v.w;
         if constexpr (VB == 3) {
-          const ba_u32x2 v1 = *reinterpret_cast<const ba_u32x2*>(tb + 1024 + 8 * lane);
+          const ba_u32x2 v1 = at(ba_u32x2{}, a.vtiles, vrs, 8u * lane, row[0], 8 * VB, 1024);
           t.vw[4] = v1.x; t.vw[5] = v1.y;
         } else if constexpr (VB == 4) {
-          const ba_u32x4 v1 = *reinterpret_cast<const ba_u32x4*>(tb + 1024 + 16 * lane);
+          const ba_u32x4 v1 = at(ba_u32x4{}, a.vtiles, vrs, 16u * lane, row[0], 8 * VB, 1024);
           t.vw[4] = v1.x; t.vw[5] = v1.y; t.vw[6] = v1.z; t.vw[7] = v1.w;
         }
       }
     };
 
-
     auto compute = [&](int i, const Tile& t) {
       const int p0 = (k0 + i) << 6;  // position of the tile's first token
-      // norms of tokens no row sees may be stale, even NaN
-      const bool live = p0 + lane >= lo_min && p0 + lane < hi_max;
-      const float nvl = live ? t.nv : 0.f;
+      const bool mask = p0 < lo_max || p0 + 64 > hi_min;
+      float nvl = t.nv;
+      bool odd = false;  // a token that not all rows see has an inf or NaN norm
+      if (__builtin_expect(mask, 0)) {
+        // norms of tokens no row sees may be stale, even NaN
+        nvl = p0 + lane >= lo_min && p0 + lane < hi_max ? t.nv : 0.f;
+        odd = __any(!(fabsf(nvl) < INFINITY));
+      }
       if (vs.over(fabsf(nvl) * vs.s)) {
         const float f = vs.rescale(fabsf(nvl));
 #pragma unroll
@@ -320,7 +330,6 @@ __global__ __launch_bounds__(kBaThreads, 2) void batch_attn_kernel(BaArgs a, BaL
       snorm[lane] = t.nk;
       snorm[64 + lane] = nvl * vs.s;
       __builtin_amdgcn_wave_barrier();
-      const bool mask = p0 < lo_max || p0 + 64 > hi_min;
 
       // value word helpers: VB 3 / 4, tile word i of half s, and the word whose bytes index
       // the pair entries of dim group nb
@@ -331,7 +340,7 @@ __global__ __launch_bounds__(kBaThreads, 2) void batch_attn_kernel(BaArgs a, BaL
           return __builtin_amdgcn_perm(t.vw[2 * (2 * s + 1) + (i2 >> 1)], t.vw[2 * (2 * s) + (i2 >> 1)],
                                        (i2 & 1) ? 0x07060302u : 0x05040100u);
         } else {
-          return i2 == 2 ? __builtin_amdgcn_perm(t.vw[4 + 2 * s + 1], t.vw[4 + 2 * s], 0x05040100u)
+          return i2 == 2 ? __builtin_amdgcn_perm(t.vw[4 + 2 * s + 1], t.vw[4 + 2 * s], vsel)
                          : __builtin_amdgcn_perm(t.vw[2 * s + 1], t.vw[2 * s], i2 ? 0x07060302u : 0x05040100u);
         }
       };
@@ -348,7 +357,7 @@ __global__ __launch_bounds__(kBaThreads, 2) void batch_attn_kernel(BaArgs a, BaL
 
       // ---- scores over the norm's and the scales' powers of two: entry k of a lane is its copy's
       // 16-token group NB cb + k
-      ba_v4f sv[NGR][NB];
+      ba_v4f sv[NGR][NB], all[NGR][4];
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         ba_v4f acc[NGR];
@@ -376,15 +385,19 @@ __global__ __launch_bounds__(kBaThreads, 2) void batch_attn_kernel(BaArgs a, BaL
           }
         }
 #pragma unroll
-        for (int j = 0; j < NGR; ++j) {
+        for (int j = 0; j < NGR; ++j) all[j][b] = acc[j];
+      }
+#pragma unroll
+      for (int j = 0; j < NGR; ++j)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
           if (b / NB == 0) {
-            sv[j][b % NB] = acc[j];
+            sv[j][b] = all[j][b];
           } else {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) sv[j][b % NB][r] = cb == b / NB ? acc[j][r] : sv[j][b % NB][r];
+            for (int r = 0; r < 4; ++r) sv[j][b % NB][r] = cb == b / NB ? all[j][b][r] : sv[j][b % NB][r];
           }
         }
-      }
       const int tg = 16 * NB * cb + 4 * g;  // the lane's first token of the tile
 #pragma unroll
       for (int k = 0; k < NB; ++k) {
@@ -452,8 +465,7 @@ __global__ __launch_bounds__(kBaThreads, 2) void batch_attn_kernel(BaArgs a, BaL
             // results below 2^-126 flush to 0: nothing beside the running maximum's 1
             const float p = __builtin_amdgcn_exp2f(fmaf(sv[j][k][r], kin, -ms));
             l[j] += p;
-            float v = p * nv4[k][r];
-            if (mask) v = p == 0.f ? 0.f : v;  // another row's inf or NaN norm
+            const float v = p * nv4[k][r];
             if constexpr (PREC) {
               _Float16 hv, lv;
               split_f16(v, hv, lv);
@@ -463,6 +475,17 @@ __global__ __launch_bounds__(kBaThreads, 2) void batch_attn_kernel(BaArgs a, BaL
               ph[k][r] = (_Float16)v;
             }
           }
+        if (__builtin_expect(odd, 0)) {  // rows that do not see it must not take 0 * inf
+          asm volatile("");
+#pragma unroll
+          for (int k = 0; k < NB; ++k)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (sv[j][k][r] == -INFINITY) {
+                ph[k][r] = (_Float16)0.f;
+                if constexpr (PREC) pl[k][r] = (_Float16)0.f;
+              }
+        }
         // the second products' operand: 16-token group b in half b % 2 of part b / 2
         const v4h zero = {(_Float16)0.f, (_Float16)0.f, (_Float16)0.f, (_Float16)0.f};
 #pragma unroll
@@ -497,10 +520,9 @@ __global__ __launch_bounds__(kBaThreads, 2) void batch_attn_kernel(BaArgs a, BaL
 #pragma unroll
         for (int nb = 0; nb < 4; ++nb) {
           ba_v8h ah, al;
-          const uint8_t* vt = smem + kBaVTab;
           if constexpr (VB == 2) {
-            const uint8_t* q0 = vt + vaddr(t.vw[2 * s], nb);
-            const uint8_t* q1 = vt + vaddr(t.vw[2 * s + 1], nb);
+            const uint8_t* q0 = smem + vaddr(t.vw[2 * s], nb);
+            const uint8_t* q1 = smem + vaddr(t.vw[2 * s + 1], nb);
             const ba_u32x2 e0 = *reinterpret_cast<const ba_u32x2*>(q0), e1 = *reinterpret_cast<const ba_u32x2*>(q1);
             ah = ba_h8(e0.x, e0.y, e1.x, e1.y);
             if constexpr (PREC) {
@@ -509,10 +531,10 @@ __global__ __launch_bounds__(kBaThreads, 2) void batch_attn_kernel(BaArgs a, BaL
             }
           } else {
             const uint32_t vw = vword(s, nb);
-            const uint8_t* q0 = vt + vaddr(vw, 0);
-            const uint8_t* q1 = vt + vaddr(vw, 1);
-            const uint8_t* q2 = vt + vaddr(vw, 2);
-            const uint8_t* q3 = vt + vaddr(vw, 3);
+            const uint8_t* q0 = smem + vaddr(vw, 0);
+            const uint8_t* q1 = smem + vaddr(vw, 1);
+            const uint8_t* q2 = smem + vaddr(vw, 2);
+            const uint8_t* q3 = smem + vaddr(vw, 3);
             ah = ba_h8(*reinterpret_cast<const uint32_t*>(q0), *reinterpret_cast<const uint32_t*>(q1),
                        *reinterpret_cast<const uint32_t*>(q2), *reinterpret_cast<const uint32_t*>(q3));
             if constexpr (PREC)
@@ -531,24 +553,8 @@ __global__ __launch_bounds__(kBaThreads, 2) void batch_attn_kernel(BaArgs a, BaL
       }
     };
 
-    if constexpr (NGR == 1) {  // three buffers, two tiles ahead; whole groups of three, then the rest
-      if (nw > 0) {
-        Tile r0, r1, r2;
-        load(0, r0);
-        load(1, r1);
-        int i = 0;
-        for (; i + 2 < nw; i += 3) {
-          load(i + 2, r2);
-          compute(i, r0);
-          load(i + 3, r0);
-          compute(i + 1, r1);
-          load(i + 4, r1);
-          compute(i + 2, r2);
-        }
-        if (i < nw) compute(i, r0);
-        if (i + 1 < nw) compute(i + 1, r1);
-      }
-    } else if (nw > 0) {  // two buffers: the third would spill, and a tile takes longer here
+    // two buffers, one tile ahead: the other waves of the SIMD cover the rest
+    if (nw > 0) {
       Tile r0, r1;
       load(0, r0);
       int i = 0;
@@ -561,8 +567,9 @@ __global__ __launch_bounds__(kBaThreads, 2) void batch_attn_kernel(BaArgs a, BaL
       if (i < nw) compute(i, r0);
     }
 
+    if (next) it = ln.items[++item];
     // ---- the piece's sums: over the row's lanes and, for few rows, its copies
-    const float vinv = vs.inv() / vsc;  // powers of two
+    const float vinv = vs.inv() * vsc_inv;
 #pragma unroll
     for (int j = 0; j < NGR; ++j) {
       l[j] += __shfl_xor(l[j], 16, 64);
@@ -590,7 +597,9 @@ __global__ __launch_bounds__(kBaThreads, 2) void batch_attn_kernel(BaArgs a, BaL
         }
       }
       if (cb == 0 && row0 + 16 * j + cr <= lastrow) {
-        const int64_t rowid = (int64_t)tok[j] * a.hq + qh[j];
+        int tok, qh;
+        place_of(j, tok, qh);
+        const int64_t rowid = (int64_t)tok * a.hq + qh;
         float* slot = ln.slots + ((int64_t)w * 2 + (ta == 0)) * ba_slot_floats(R);
         float* sums = whole ? ln.row_sums + rowid * 64 : slot + (16 * j + cr) * 64;
         float* st = whole ? ln.row_stats + rowid * 2 : slot + R * 64 + (16 * j + cr) * 2;
@@ -605,25 +614,25 @@ __global__ __launch_bounds__(kBaThreads, 2) void batch_attn_kernel(BaArgs a, BaL
   }
 }
 
-template <int VB, bool SUB, bool PREC>
+template <int VB, bool SUB, bool PREC, bool WIDE>
 void ba_launch_kind(const BaArgs& a, int l, int rw, int groups, unsigned grid, hipStream_t st) {
   constexpr int N = ba_groups(PREC);
-  const dim3 gr(grid), bl(kBaThreads);
+  const dim3 gr(grid), bl(64 * ba_waves(PREC, rw, groups));
   const BaLine& ln = a.line[l];
-  if (groups > 1) hipLaunchKernelGGL((batch_attn_kernel<VB, SUB, PREC, 16, N>), gr, bl, 0, st, a, ln);
-  else if (rw == 16) hipLaunchKernelGGL((batch_attn_kernel<VB, SUB, PREC, 16, 1>), gr, bl, 0, st, a, ln);
-  else if (rw == 8) hipLaunchKernelGGL((batch_attn_kernel<VB, SUB, PREC, 8, 1>), gr, bl, 0, st, a, ln);
-  else hipLaunchKernelGGL((batch_attn_kernel<VB, SUB, PREC, 4, 1>), gr, bl, 0, st, a, ln);
+  if (groups > 1) hipLaunchKernelGGL((batch_attn_kernel<VB, SUB, PREC, 16, N, WIDE>), gr, bl, 0, st, a, ln);
+  else if (rw == 16) hipLaunchKernelGGL((batch_attn_kernel<VB, SUB, PREC, 16, 1, WIDE>), gr, bl, 0, st, a, ln);
+  else if (rw == 8) hipLaunchKernelGGL((batch_attn_kernel<VB, SUB, PREC, 8, 1, WIDE>), gr, bl, 0, st, a, ln);
+  else hipLaunchKernelGGL((batch_attn_kernel<VB, SUB, PREC, 4, 1, WIDE>), gr, bl, 0, st, a, ln);
 }
 
 }  // namespace
 
-template <int VB>
-void ba_launch(const BaArgs& a, int l, bool sub, bool prec, int rw, int groups, unsigned grid, hipStream_t st) {
-  if (sub && prec) ba_launch_kind<VB, true, true>(a, l, rw, groups, grid, st);
-  else if (sub) ba_launch_kind<VB, true, false>(a, l, rw, groups, grid, st);
-  else if (prec) ba_launch_kind<VB, false, true>(a, l, rw, groups, grid, st);
-  else ba_launch_kind<VB, false, false>(a, l, rw, groups, grid, st);
+template <int VB, bool SUB>
+void ba_launch(const BaArgs& a, int l, bool wide, bool prec, int rw, int groups, unsigned grid, hipStream_t st) {
+  if (wide && prec) ba_launch_kind<VB, SUB, true, true>(a, l, rw, groups, grid, st);
+  else if (wide) ba_launch_kind<VB, SUB, false, true>(a, l, rw, groups, grid, st);
+  else if (prec) ba_launch_kind<VB, SUB, true, false>(a, l, rw, groups, grid, st);
+  else ba_launch_kind<VB, SUB, false, false>(a, l, rw, groups, grid, st);
 }
 
 }  // namespace tq
