@@ -701,6 +701,7 @@ typedef struct tq_score_variant {
  * [n_groups]): the tables of a group's sequences all begin with the blocks of its first
  * shared_lens tokens, which are then read once for all the group's rows, through its first
  * sequence's table.  Results are those without groups, to rounding.
+ * transposed: bit 0 (1): krotation (vrotation) is stored column by column.
  * Replaces the reference backend's attention (vllm_plugin/__init__.py:400), whose Impl takes
  * alibi_slopes, sliding_window and logits_soft_cap and applies none of them.
  * Positions past max_blocks * block_size hold no tokens; block ids are clamped into the pool.
@@ -719,9 +720,9 @@ int tq_attention_batch_paged_dl(const void* q, tq_dtype q_dtype, int32_t n_token
                                 const int32_t* seq_lens, int32_t n_seqs,
                                 const int32_t* group_start_loc, const int32_t* shared_lens,
                                 int32_t n_groups, const float* kcentroids, const float* vcentroids,
-                                const float* krotation, const float* vrotation, float scale,
-                                const tq_score_variant* variant, void* out, int64_t out_stride,
-                                int32_t zero_tail, float* lse, void* workspace,
+                                const float* krotation, const float* vrotation,
+                                int32_t transposed, float scale, const tq_score_variant* variant,
+                                void* out, int64_t out_stride, int32_t zero_tail, float* lse, void* workspace,
                                 size_t workspace_bytes, void* stream);
 
 /*

@@ -1343,8 +1343,13 @@ std::tuple<at::Tensor, at::Tensor> attention_batch(
   TORCH_CHECK(qs.numel() == B + 1, "query_start_loc must have num_seqs + 1 entries");
   auto kc = f32c(kcentroids, dev);
   auto vc = f32c(vcentroids, dev);
-  auto Rk = f32c(krotation, dev);
-  auto Rv = f32c(vrotation, dev);
+  // rotations stored column by column (as factorizations give them) are read in place
+  const auto by_column = [&](const at::Tensor& r) {
+    return r.dim() == 2 && r.scalar_type() == at::kFloat && r.device() == dev && !r.is_contiguous() && r.t().is_contiguous();
+  };
+  const int transposed = (by_column(krotation) ? 1 : 0) | (by_column(vrotation) ? 2 : 0);
+  auto Rk = transposed & 1 ? krotation : f32c(krotation, dev);
+  auto Rv = transposed & 2 ? vrotation : f32c(vrotation, dev);
   TORCH_CHECK(kc.numel() == 16 && vc.numel() == (1 << vb),
               "decode layout: 4-bit keys (16 centroids) and 2^VB value centroids for the pool's "
               "VB-bit value tiles");
@@ -1396,7 +1401,7 @@ std::tuple<at::Tensor, at::Tensor> attention_batch(
       vnorm_pool.data_ptr<float>(), nb, (int32_t)bs, (int32_t)vb, bt.data_ptr<int32_t>(), bt.size(1),
       (int32_t)bt.size(1), qs.data_ptr<int32_t>(), sl.data_ptr<int32_t>(), (int32_t)B,
       ng ? groups.data_ptr<int32_t>() : nullptr, ng ? shared.data_ptr<int32_t>() : nullptr, (int32_t)ng,
-      kc.data_ptr<float>(), vc.data_ptr<float>(), Rk.data_ptr<float>(), Rv.data_ptr<float>(), (float)scale, &v,
+      kc.data_ptr<float>(), vc.data_ptr<float>(), Rk.data_ptr<float>(), Rv.data_ptr<float>(), transposed, (float)scale, &v,
       out.data_ptr(), n <= 1 ? Hq * d : out.stride(0), into.has_value() ? 0 : 1,
       want_lse ? lse.data_ptr<float>() : nullptr, ws.data_ptr(), ws.numel(), cur_stream(qq)));
   return {out, lse};

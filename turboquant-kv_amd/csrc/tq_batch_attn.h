@@ -53,8 +53,7 @@ namespace tq {
 constexpr int ba_waves(bool prec, int rw, int groups) { return prec && groups == 1 && rw < 16 ? 12 : 8; }
 constexpr int kBaMaxSegs = 8191;  // sequences or groups of a call: the preparing kernel's LDS
 constexpr int kBaOver = 3;        // an (item, head)'s cost besides its tiles, in tiles
-// Row groups of a wave where rows abound: with hi + lo parts two fit the registers.
-constexpr int ba_groups(bool prec) { return prec ? 2 : 3; }
+constexpr int kBaGroups = 2;      // groups of 16 rows a wave takes where rows abound: three spill
 // Floats of a partial slot of R rows: sums [R][64], (maximum, sum) [R][2].
 constexpr int ba_slot_floats(int R) { return R * 66; }
 
@@ -118,6 +117,7 @@ struct BaArgs {
   const float* vcen;
   const float* krot;
   const float* vrot;
+  int krot_row, krot_col, vrot_row, vrot_col;  // strides of their rows and columns
   float qscale;                // softmax scale * log2(e)
   float cap2, cap2_inv;        // softcap * log2(e) and its inverse, or 0
   const float* slopes;         // [hq] or null
@@ -133,6 +133,8 @@ struct BaArgs {
   _Float16* qlo;               // and lo parts (fp32 / fp16 queries)
   float* qscale_inv;           // [n_tokens * hq] what undoes it and the key centroids' scale
   BaEntry* entries;            // [256]
+  _Float16* vrot16;            // R_v's operands, [2 parts][4 ob][2 s][64 lanes][8]: see ba_rotate_back
+  int direct;                  // (no groups) waves write the results of whole items of many rows
   BaToken* tokens;             // [n_tokens]
   BaLine line[2];              // sequences, groups
 };
@@ -171,6 +173,63 @@ __device__ __forceinline__ int ba_last(int n, int v, F key) {
 // a / b for 0 <= a, 0 < b: places rarely need 64 bits, whose division takes ten times as long.
 __device__ __forceinline__ int64_t ba_div(int64_t a, int64_t b) {
   return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
+
+// The rows' results from their sums: out_c[16 ob + 4 g + r] of lane (c, g), c the row, in fp16
+// products over 32 dims: part s's operands are A[c][8 g + i] = R_v[dim][16 ob + c] and B[8 g + i][c]
+// = x_c[dim] with dim = 16 (2 s + i / 4) + 4 g + i % 4, the dims that lane (c, g) holds in
+// x[2 s + i / 4][i % 4].  PREC: hi + lo parts of both.  |x| at most 2^15.
+template <bool PREC>
+__device__ __forceinline__ void ba_rotate_back(const _Float16* vrot16, const ba_v4f* x, int lane, ba_v4f* out) {
+  ba_v8h hi[2], lo[2];
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (PREC) {
+        _Float16 hv, lv;
+        split_f16(x[2 * s + (i >> 2)][i & 3], hv, lv);
+        hi[s][i] = hv;
+        lo[s][i] = lv;
+      } else {
+        hi[s][i] = (_Float16)x[2 * s + (i >> 2)][i & 3];
+      }
+    }
+  if constexpr (PREC) mfma_operand_fence(hi[0], hi[1], lo[0], lo[1]);
+  else mfma_operand_fence(hi[0], hi[1]);
+#pragma unroll
+  for (int ob = 0; ob < 4; ++ob) {
+    out[ob] = (ba_v4f){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const ba_v8h* src = reinterpret_cast<const ba_v8h*>(vrot16) + (ob * 2 + s) * 64 + lane;
+      const ba_v8h ah = src[0];
+      out[ob] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, hi[s], out[ob], 0, 0, 0);
+      if constexpr (PREC) {
+        const ba_v8h al = src[512];
+        out[ob] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, lo[s], out[ob], 0, 0, 0);
+        out[ob] = __builtin_amdgcn_mfma_f32_16x16x32_f16(al, hi[s], out[ob], 0, 0, 0);
+      }
+    }
+  }
+}
+
+// Four dims of a row's result, in the output's type.
+__device__ __forceinline__ void ba_store(const BaArgs& a, int tok, int qh, int dim, ba_v4f x) {
+  const int64_t at = (int64_t)tok * a.out_stride + qh * 64 + dim;
+  if (a.q_dt == TQ_F32) {
+    *reinterpret_cast<ba_v4f*>(static_cast<float*>(a.out) + at) = x;
+  } else if (a.q_dt == TQ_BF16) {
+    typedef __bf16 b4_t __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<b4_t*>(static_cast<uint16_t*>(a.out) + at) = __builtin_convertvector(x, b4_t);
+  } else {
+    typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<h4_t*>(static_cast<uint16_t*>(a.out) + at) = __builtin_convertvector(x, h4_t);
+  }
+}
+
+__device__ __forceinline__ float ba_lse(float m, float l) {
+  return l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
 }
 
 // Tiles of an (item, head) before place `place` of it.

@@ -198,11 +198,156 @@ __device__ __forceinline__ BaEntry ba_entry(const BaArgs& a, int vbits, int e, i
   return x;
 }
 
-// Workgroups 0 .. n_lines - 1 lay the lines out; the others rotate 16 rows (a token's head
-// each) a wave: Qrot = (q * qscale) R_k^T by v_mfma_f32_16x16x4f32, scaled by a power of two
-// into [0.5, 1) and split into fp16 hi (and lo) parts, and find their tokens' positions.
-__global__ __launch_bounds__(kPrepThreads) void batch_prep_kernel(BaArgs a, int n_lines, int prec, int vbits) {
+// The tables' entries and R_v's operands (one workgroup).
+__device__ __forceinline__ void ba_make_tables(const BaArgs& a, int vbits) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int ke = ba_exponent(wave_max(lane < 16 ? fabsf(a.kcen[lane]) : 0.f));
+  const int ve = ba_exponent(wave_max(lane < (1 << vbits) ? fabsf(a.vcen[lane]) : 0.f));
+  if (tid < 256) a.entries[tid] = ba_entry(a, vbits, tid, ke, ve);
+  const int c = lane & 15, g = lane >> 4, ob = tid >> 7, s = tid >> 6 & 1;
+  ba_v8h hi, lo;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float v = a.vrot[(16 * (2 * s + (i >> 2)) + 4 * g + (i & 3)) * a.vrot_row + (16 * ob + c) * a.vrot_col];
+    hi[i] = (_Float16)v;
+    lo[i] = (_Float16)(v - (float)hi[i]);
+  }
+  static_assert(kPrepThreads == 512, "a thread per lane of the eight operands");
+  reinterpret_cast<ba_v8h*>(a.vrot16)[tid] = hi;
+  reinterpret_cast<ba_v8h*>(a.vrot16)[512 + tid] = lo;
+}
+
+// The position range of token t (see BaToken).
+__device__ __forceinline__ void ba_find_token(const BaArgs& a, int t) {
+  BaToken x{0, 0, 0, a.B};
+  if (a.B > 0 && t >= ba_qs(a, 0) && t < ba_qs(a, a.B)) {
+    // token t of a step of single tokens belongs to sequence t
+    const int b = t < a.B && ba_qs(a, t) <= t && ba_qs(a, t + 1) > t
+                      ? t : ba_last(a.B, t, [&](int i) { return ba_qs(a, i); });
+    const int q0 = ba_qs(a, b), T = max(0, a.seq_lens[b]);
+    const int64_t p = (int64_t)T - (ba_qs(a, b + 1) - q0) + (t - q0);
+    int64_t lo = 0;
+    if (a.window > 0) lo = max<int64_t>(lo, p + 1 - a.window);
+    if (a.token_starts) lo = max<int64_t>(lo, a.token_starts[t]);
+    x.lo = (int)lo;
+    x.hi = (int)min<int64_t>(min(T, a.cap), max<int64_t>(p + 1, a.prefix_lens ? a.prefix_lens[b] : 0));
+    x.pos = (int)p;
+    x.seq = b;
+  }
+  a.tokens[t] = x;
+}
+
+// Workgroups 0 .. n_lines - 1 lay the lines out, the next makes the tables, the others rotate
+// 16 rows (a token's head each) a wave and round: Qrot = q R_k^T qscale, scaled by a power of
+// two into [0.5, 1) and split into fp16 hi (and lo) parts.  Lane (c, g) ends with dims 16 g ..
+// 16 g + 15 of row c, the order in which its key bytes come: output 4 k + r of product mb is
+// dim 16 k + 4 mb + r.
+//   float32 queries: v_mfma_f32_16x16x4f32, 64 products of 8 passes a round.
+//   16-bit queries: v_mfma_f32_16x16x32 on the queries as they are; R_k, held in registers over
+//   the rounds, in three bfloat16 or two float16 parts (times 2^10: none is subnormal), which
+//   carry 24 and 22 bits: 24 or 16 products of 4 passes.
+template <int DT>
+__device__ __forceinline__ void ba_rotate_rows(const BaArgs& a, int64_t blk, int64_t n_blks) {
 #pragma clang fp contract(off)
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int c = lane & 15, g = lane >> 4;
+  const int64_t n_rows = (int64_t)a.n_tokens * a.hq;
+  const int ke = ba_exponent(wave_max(lane < 16 ? fabsf(a.kcen[lane]) : 0.f));
+  constexpr int PARTS = DT == TQ_BF16 ? 3 : 2;
+  typedef __bf16 v8b __attribute__((ext_vector_type(8)));
+  using v8 = std::conditional_t<DT == TQ_BF16, v8b, ba_v8h>;
+  using elem = std::conditional_t<DT == TQ_BF16, __bf16, _Float16>;
+  constexpr float kUp = DT == TQ_F16 ? 1024.f : 1.f;
+  v8 part[DT == TQ_F32 ? 1 : PARTS][4][2];
+  if constexpr (DT != TQ_F32) {
+#pragma unroll
+    for (int mb = 0; mb < 4; ++mb)
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          float v = kUp * a.krot[(16 * (c >> 2) + 4 * mb + (c & 3)) * a.krot_row + (32 * s + 8 * g + i) * a.krot_col];
+#pragma unroll
+          for (int p = 0; p < PARTS; ++p) {
+            const elem x = (elem)v;
+            part[p][mb][s][i] = x;
+            v -= (float)x;
+          }
+        }
+  }
+  for (int64_t r0 = (blk * kPrepWaves + wave) * 16; r0 < n_rows; r0 += n_blks * kPrepWaves * 16) {
+    const int64_t row = min(r0 + c, n_rows - 1);
+    const int64_t qt = ba_div(row, a.hq), qo = qt * a.q_stride + (row - qt * a.hq) * 64;
+    ba_v4f d[4];
+    if constexpr (DT == TQ_F32) {
+      float qv[16];
+      const ba_v4f* src = reinterpret_cast<const ba_v4f*>(static_cast<const float*>(a.q) + qo + 16 * g);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const ba_v4f v = src[i];
+        qv[4 * i] = v.x; qv[4 * i + 1] = v.y; qv[4 * i + 2] = v.z; qv[4 * i + 3] = v.w;
+      }
+#pragma unroll
+      for (int mb = 0; mb < 4; ++mb) {
+        float rk[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          rk[i] = a.krot[(16 * (c >> 2) + 4 * mb + (c & 3)) * a.krot_row + (16 * g + i) * a.krot_col];
+        d[mb] = (ba_v4f){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 16; ++i) d[mb] = __builtin_amdgcn_mfma_f32_16x16x4f32(rk[i], qv[i], d[mb], 0, 0, 0);
+      }
+    } else {
+      v8 q8[2];
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        q8[s] = *reinterpret_cast<const v8*>(static_cast<const uint16_t*>(a.q) + qo + 32 * s + 8 * g);
+#pragma unroll
+      for (int mb = 0; mb < 4; ++mb) {
+        d[mb] = (ba_v4f){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int p = PARTS - 1; p >= 0; --p)  // the small parts first
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            if constexpr (DT == TQ_BF16) d[mb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(part[p][mb][s], q8[s], d[mb], 0, 0, 0);
+            else d[mb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(part[p][mb][s], q8[s], d[mb], 0, 0, 0);
+          }
+      }
+    }
+    float qm = 0.f;
+#pragma unroll
+    for (int mb = 0; mb < 4; ++mb)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        d[mb][r] *= a.qscale * (1.f / kUp);
+        qm = fmaxf(qm, fabsf(d[mb][r]));
+      }
+    qm = fmaxf(qm, __shfl_xor(qm, 16, 64));
+    qm = fmaxf(qm, __shfl_xor(qm, 32, 64));
+    const int e = ba_exponent(qm);
+    const float qsc = ldexpf(1.f, -e);
+    ba_v8h hi[2], lo[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float v = d[2 * s + (i >> 2)][i & 3] * qsc;
+        hi[s][i] = (_Float16)v;
+        lo[s][i] = (_Float16)(v - (float)hi[s][i]);
+      }
+    if (r0 + c < n_rows) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        *reinterpret_cast<ba_v8h*>(a.qhi + row * 64 + 16 * g + 8 * s) = hi[s];
+        if constexpr (DT != TQ_BF16) *reinterpret_cast<ba_v8h*>(a.qlo + row * 64 + 16 * g + 8 * s) = lo[s];
+      }
+      if (g == 0) a.qscale_inv[row] = ldexpf(1.f, e + ke);
+    }
+  }
+}
+
+template <int DT>
+__global__ __launch_bounds__(kPrepThreads) void batch_prep_kernel(BaArgs a, int n_lines, int vbits) {
   __shared__ int32_t base_s[kBaMaxSegs + 2];
   __shared__ int64_t start_s[kPrepStarts];
   __shared__ int64_t part[kPrepWaves];
@@ -211,103 +356,13 @@ __global__ __launch_bounds__(kPrepThreads) void batch_prep_kernel(BaArgs a, int 
     else ba_lay_out<1>(a, base_s, start_s, part);
     return;
   }
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int c = lane & 15, g = lane >> 4;
-  const int64_t blk = (int)blockIdx.x - n_lines;
-  const int64_t n_rows = (int64_t)a.n_tokens * a.hq;
-  // ---- positions of token `t`
-  const int64_t t64 = blk * kPrepThreads + tid;
-  if (t64 < a.n_tokens) {
-    const int t = (int)t64;
-    BaToken x{0, 0, 0, a.B};
-    if (a.B > 0 && t >= ba_qs(a, 0) && t < ba_qs(a, a.B)) {
-      // token t of a step of single tokens belongs to sequence t
-      const int b = t < a.B && ba_qs(a, t) <= t && ba_qs(a, t + 1) > t
-                        ? t : ba_last(a.B, t, [&](int i) { return ba_qs(a, i); });
-      const int q0 = ba_qs(a, b), T = max(0, a.seq_lens[b]);
-      const int64_t p = (int64_t)T - (ba_qs(a, b + 1) - q0) + (t - q0);
-      int64_t lo = 0;
-      if (a.window > 0) lo = max<int64_t>(lo, p + 1 - a.window);
-      if (a.token_starts) lo = max<int64_t>(lo, a.token_starts[t]);
-      x.lo = (int)lo;
-      x.hi = (int)min<int64_t>(min(T, a.cap), max<int64_t>(p + 1, a.prefix_lens ? a.prefix_lens[b] : 0));
-      x.pos = (int)p;
-      x.seq = b;
-    }
-    a.tokens[t] = x;
+  const int64_t blk = (int64_t)blockIdx.x - n_lines - 1, n_blks = (int64_t)gridDim.x - n_lines - 1;
+  if (blk < 0) {
+    ba_make_tables(a, vbits);
+    return;
   }
-  // ---- the centroids' scales; the tables' entries (once)
-  const int ke = ba_exponent(wave_max(lane < 16 ? fabsf(a.kcen[lane]) : 0.f));
-  if (blk == 0 && tid < 256) {
-    const int ve = ba_exponent(wave_max(lane < (1 << vbits) ? fabsf(a.vcen[lane]) : 0.f));
-    a.entries[tid] = ba_entry(a, vbits, tid, ke, ve);
-  }
-  // ---- rows.  MFMA mb, k-step s: lane (c, g) supplies A[c][g] = R_k[16 (c / 4) + 4 mb + c % 4][16 g + s]
-  // and B[g][c] = q_c[16 g + s]; register r of lane (c, g) gets Qrot_c[16 g + 4 mb + r]: a lane
-  // ends with dims 16 g .. 16 g + 15, the order in which its key bytes come.
-  const int64_t r0 = (blk * kPrepWaves + wave) * 16;
-  if (r0 >= n_rows) return;
-  const int64_t row = min(r0 + c, n_rows - 1);
-  const int64_t qt = ba_div(row, a.hq), qo = qt * a.q_stride + (row - qt * a.hq) * 64 + 16 * g;
-  float qv[16];
-  if (a.q_dt == TQ_F32) {
-    const ba_v4f* src = reinterpret_cast<const ba_v4f*>(static_cast<const float*>(a.q) + qo);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const ba_v4f v = src[i];
-      qv[4 * i] = v.x; qv[4 * i + 1] = v.y; qv[4 * i + 2] = v.z; qv[4 * i + 3] = v.w;
-    }
-  } else {
-    const ba_u32x4* src = reinterpret_cast<const ba_u32x4*>(static_cast<const uint16_t*>(a.q) + qo);
-    const bool bf = a.q_dt == TQ_BF16;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const ba_u32x4 v = src[i];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint32_t hb = (v[e >> 1] >> (16 * (e & 1))) & 0xFFFFu;
-        qv[8 * i + e] = bf ? __uint_as_float(hb << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)hb);
-      }
-    }
-  }
-  ba_v4f d[4];
-#pragma unroll
-  for (int mb = 0; mb < 4; ++mb) {
-    const ba_v4f* src = reinterpret_cast<const ba_v4f*>(a.krot + (16 * (c >> 2) + 4 * mb + (c & 3)) * 64 + 16 * g);
-    d[mb] = (ba_v4f){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const ba_v4f rk = src[i];
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        d[mb] = __builtin_amdgcn_mfma_f32_16x16x4f32(rk[e], qv[4 * i + e] * a.qscale, d[mb], 0, 0, 0);
-    }
-  }
-  float qm = 0.f;
-#pragma unroll
-  for (int mb = 0; mb < 4; ++mb)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) qm = fmaxf(qm, fabsf(d[mb][r]));
-  qm = fmaxf(qm, __shfl_xor(qm, 16, 64));
-  qm = fmaxf(qm, __shfl_xor(qm, 32, 64));
-  const int e = ba_exponent(qm);
-  const float qsc = ldexpf(1.f, -e);
-  ba_v8h hi[2], lo[2];
-#pragma unroll
-  for (int s = 0; s < 2; ++s)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float v = d[2 * s + (i >> 2)][i & 3] * qsc;
-      hi[s][i] = (_Float16)v;
-      lo[s][i] = (_Float16)(v - (float)hi[s][i]);
-    }
-  if (r0 + c >= n_rows) return;
-#pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    *reinterpret_cast<ba_v8h*>(a.qhi + row * 64 + 16 * g + 8 * s) = hi[s];
-    if (prec) *reinterpret_cast<ba_v8h*>(a.qlo + row * 64 + 16 * g + 8 * s) = lo[s];
-  }
-  if (g == 0) a.qscale_inv[row] = ldexpf(1.f, e + ke);
+  for (int64_t t = blk * kPrepThreads + threadIdx.x; t < a.n_tokens; t += n_blks * kPrepThreads) ba_find_token(a, (int)t);
+  ba_rotate_rows<DT>(a, blk, n_blks);
 }
 
 // ------------------------------------------------------------------------------- joining
@@ -359,7 +414,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void batch_join_kernel(BaArgs a) {
 #pragma unroll
   for (int nb = 0; nb < 4; ++nb)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) rv[4 * nb + r] = a.vrot[(16 * nb + 4 * g + r) * 64 + 16 * wave + c];
+    for (int r = 0; r < 4; ++r) rv[4 * nb + r] = a.vrot[(16 * nb + 4 * g + r) * a.vrot_row + (16 * wave + c) * a.vrot_col];
 
   const BaToken t = a.tokens[tok];
   BaFrom s{}, p{};
@@ -431,20 +486,79 @@ __global__ __launch_bounds__(64 * kJoinWaves) void batch_join_kernel(BaArgs a) {
     for (int r = 0; r < 4; ++r) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(rv[4 * nb + r], x[r] * inv, acc, 0, 0, 0);
   }
   if (r0 + c >= n_rows) return;
-  if (t.seq < a.B || a.zero_tail) {
-    const int64_t oa = (int64_t)tok * a.out_stride + qh * 64 + 16 * wave + 4 * g;
-    if (a.q_dt == TQ_F32) {
-      *reinterpret_cast<ba_v4f*>(static_cast<float*>(a.out) + oa) = acc;
-    } else if (a.q_dt == TQ_BF16) {
-      typedef __bf16 b4_t __attribute__((ext_vector_type(4)));
-      *reinterpret_cast<b4_t*>(static_cast<uint16_t*>(a.out) + oa) = __builtin_convertvector(acc, b4_t);
-    } else {
-      typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
-      *reinterpret_cast<h4_t*>(static_cast<uint16_t*>(a.out) + oa) = __builtin_convertvector(acc, h4_t);
+  if (t.seq < a.B || a.zero_tail) ba_store(a, tok, qh, 16 * wave + 4 * g, acc);
+  if (a.lse && wave == 0 && g == 0) a.lse[rowid] = ba_lse(M, L);
+}
+
+// Where waves write whole items themselves: workgroup (w, j) joins group j of the (item, head)
+// that the border before wave w's piece cuts, if it is that one's first border; the last
+// kTailBlocks workgroups write the rows behind the last sequence.  A wave rotates a quarter of the
+// dims; all four read the sums of the waves that took a part.
+constexpr int kTailBlocks = 32;
+template <bool PREC>
+__global__ __launch_bounds__(64) void batch_join_cut_kernel(BaArgs a) {
+#pragma clang fp contract(off)
+  const BaLine& ln = a.line[0];
+  const int lane = threadIdx.x, c = lane & 15, g = lane >> 4;
+  const int groups = ln.rows / 16;
+  const int w = (int)(blockIdx.x / (unsigned)groups) + 1, j = (int)(blockIdx.x % (unsigned)groups);
+  if (w >= ln.waves) {
+    const int first = a.B > 0 ? ba_qs(a, a.B) : 0, head = a.B > 0 ? ba_qs(a, 0) : 0;
+    const int64_t n = (int64_t)(a.n_tokens - first + head) * a.hq;
+    for (int64_t i = (int64_t)(blockIdx.x - (unsigned)(groups * (ln.waves - 1))) * 4 + g; i < n; i += kTailBlocks * 4) {
+      const int t = (int)ba_div(i, a.hq), qh = (int)(i - (int64_t)t * a.hq);
+      const int tok = t < head ? t : first + t - head;
+      if (a.zero_tail) ba_store(a, tok, qh, 4 * c, (ba_v4f){0.f, 0.f, 0.f, 0.f});
+      if (a.lse && c == 0) a.lse[(int64_t)tok * a.hq + qh] = -INFINITY;
     }
+    return;
   }
-  if (a.lse && wave == 0 && g == 0)
-    a.lse[rowid] = L == 0.f ? -INFINITY : (M + __builtin_amdgcn_logf(L)) * 0.6931471805599453f;
+  const int64_t chunk = ln.head->chunk, p = w * chunk;
+  if (p >= ln.head->total) return;
+  const BaItem it = ln.items[ln.work[w]];
+  const int64_t cost = it.nt + kBaOver;
+  const int h = (int)ba_div(p - it.start, cost);
+  const int64_t start = it.start + h * cost;
+  const int64_t w0 = ba_div(start + kBaOver, chunk), w1 = ba_div(start + cost - 1, chunk);
+  const int row = it.row0 + 16 * j + c;
+  if (w0 == w1 || it.nt == 0 || w != (int)w0 + 1 || it.row0 + 16 * j >= it.nrows) return;
+  float m = -INFINITY, l = 0.f;
+  ba_v4f x[4], out[4];
+#pragma unroll
+  for (int nb = 0; nb < 4; ++nb) x[nb] = (ba_v4f){0.f, 0.f, 0.f, 0.f};
+  for (int64_t k = w0; k <= w1; ++k) {
+    const float* slot = ln.slots + (k * 2 + (k == w0)) * ba_slot_floats(ln.rows);
+    const float* sums = slot + (16 * j + c) * 64;
+    const float* st = slot + ln.rows * 64 + (16 * j + c) * 2;
+    const float mi = st[0], li = st[1];
+    const float mn = fmaxf(m, mi), ms = mn == -INFINITY ? 0.f : mn;
+    const float fa = __builtin_amdgcn_exp2f(m - ms), fb = __builtin_amdgcn_exp2f(mi - ms);
+    m = mn;
+    l = l * fa + li * fb;
+#pragma unroll
+    for (int nb = 0; nb < 4; ++nb)
+      x[nb] = x[nb] * fa + *reinterpret_cast<const ba_v4f*>(sums + 16 * nb + 4 * g) * fb;
+  }
+  // into fp16's range by a power of two of the row
+  float xm = 0.f;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int nb = 0; nb < 4; ++nb) {
+    x[nb] *= inv;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) xm = fmaxf(xm, fabsf(x[nb][r]));
+  }
+  xm = fmaxf(xm, __shfl_xor(xm, 16, 64));
+  xm = fmaxf(xm, __shfl_xor(xm, 32, 64));
+  const int e = ba_exponent(xm);
+#pragma unroll
+  for (int nb = 0; nb < 4; ++nb) x[nb] *= ldexpf(1.f, 4 - e);
+  ba_rotate_back<PREC>(a.vrot16, x, lane, out);
+  if (row >= it.nrows) return;
+  const int ti = row / a.G, tok = it.tok0 + ti, qh = h * a.G + (row - ti * a.G);
+#pragma unroll
+  for (int ob = 0; ob < 4; ++ob) ba_store(a, tok, qh, 16 * ob + 4 * g, out[ob] * ldexpf(1.f, e - 4));
+  if (a.lse && g == 0) a.lse[(int64_t)tok * a.hq + qh] = ba_lse(m, l);
 }
 
 // --------------------------------------------------------------------------------- plans
@@ -471,7 +585,7 @@ BaPlan ba_plan(tq_dtype q_dtype, int64_t n, int hq, int hkv, int64_t B, int64_t 
     // (whole tokens: a few rows of padding behind single tokens do not widen them)
     const int64_t avg = std::max<int64_t>(1, n / std::max<int64_t>(l ? n_groups : B, 1)) * G;
     p.rw[l] = avg <= 4 ? 4 : avg <= 8 ? 8 : 16;
-    p.groups[l] = avg <= 16 ? 1 : ba_groups(p.prec);
+    p.groups[l] = avg <= 16 ? 1 : kBaGroups;
     const int R = p.rw[l] * p.groups[l];
     p.items[l] = rows / R + p.segs[l];
     // one workgroup per CU, fewer where even one-tile pieces would not fill them
@@ -495,6 +609,7 @@ size_t ba_place(const BaPlan& p, int64_t n, int hq, char* at, BaArgs* a) {
   b.tokens = reinterpret_cast<BaToken*>(take(n * sizeof(BaToken)));
   b.qscale_inv = reinterpret_cast<float*>(take(rows * 4));
   b.qhi = reinterpret_cast<_Float16*>(take(rows * 128));
+  b.vrot16 = reinterpret_cast<_Float16*>(take(2 * 4096 * sizeof(_Float16)));
   if (p.prec) b.qlo = reinterpret_cast<_Float16*>(take(rows * 128));
   for (int l = 0; l < 2; ++l) {
     if (p.grid[l] == 0) continue;
@@ -511,7 +626,7 @@ size_t ba_place(const BaPlan& p, int64_t n, int hq, char* at, BaArgs* a) {
     ln.row_stats = reinterpret_cast<float*>(take(rows * 8));
   }
   if (a) {
-    a->entries = b.entries; a->tokens = b.tokens; a->qscale_inv = b.qscale_inv; a->qhi = b.qhi; a->qlo = b.qlo;
+    a->entries = b.entries; a->vrot16 = b.vrot16; a->tokens = b.tokens; a->qscale_inv = b.qscale_inv; a->qhi = b.qhi; a->qlo = b.qlo;
     a->line[0] = b.line[0]; a->line[1] = b.line[1];
   }
   return used;
@@ -551,7 +666,7 @@ int tq_attention_batch_paged_dl(const void* q, tq_dtype q_dtype, int32_t n_token
                                 const int32_t* seq_lens, int32_t n_seqs, const int32_t* group_start_loc,
                                 const int32_t* shared_lens, int32_t n_groups, const float* kcentroids,
                                 const float* vcentroids, const float* krotation, const float* vrotation,
-                                float scale, const tq_score_variant* variant, void* out, int64_t out_stride,
+                                int32_t transposed, float scale, const tq_score_variant* variant, void* out, int64_t out_stride,
                                 int32_t zero_tail, float* lse, void* workspace, size_t workspace_bytes,
                                 void* stream) {
   TQ_REQUIRE(valid_dtype(q_dtype), "unknown dtype");
@@ -610,6 +725,8 @@ int tq_attention_batch_paged_dl(const void* q, tq_dtype q_dtype, int32_t n_token
   a.max_blocks = max_blocks; a.bs_log2 = bsl; a.num_blocks = (uint32_t)num_blocks;
   a.cap = empty ? 0 : (int)cap;
   a.kcen = kcentroids; a.vcen = vcentroids; a.krot = krotation; a.vrot = vrotation;
+  a.krot_row = transposed & 1 ? 1 : 64; a.krot_col = transposed & 1 ? 64 : 1;
+  a.vrot_row = transposed & 2 ? 1 : 64; a.vrot_col = transposed & 2 ? 64 : 1;
   a.qscale = scale * 1.4426950408889634f;
   if (v.softcap > 0.f) {
     a.cap2 = v.softcap * 1.4426950408889634f;
@@ -620,14 +737,25 @@ int tq_attention_batch_paged_dl(const void* q, tq_dtype q_dtype, int32_t n_token
   hipStream_t st = as_stream(stream);
   const int lines = n_groups > 0 ? 2 : 1;
   const int64_t qrows = (int64_t)n_tokens * hq;
-  hipLaunchKernelGGL(batch_prep_kernel, dim3((unsigned)(lines + (qrows + 16 * kPrepWaves - 1) / (16 * kPrepWaves))),
-                     dim3(kPrepThreads), 0, st, a, lines, p.prec ? 1 : 0, vbits);
+  a.direct = n_groups == 0 && p.groups[0] > 1;
+  // waves of several rounds share R_k's parts: about two workgroups a CU at the most
+  const int64_t rot = std::min<int64_t>((qrows + 16 * kPrepWaves - 1) / (16 * kPrepWaves), 2 * device_cu_count());
+  const dim3 prep((unsigned)(lines + 1 + rot)), pthreads(kPrepThreads);
+  if (q_dtype == TQ_F32) hipLaunchKernelGGL((batch_prep_kernel<TQ_F32>), prep, pthreads, 0, st, a, lines, vbits);
+  else if (q_dtype == TQ_F16) hipLaunchKernelGGL((batch_prep_kernel<TQ_F16>), prep, pthreads, 0, st, a, lines, vbits);
+  else hipLaunchKernelGGL((batch_prep_kernel<TQ_BF16>), prep, pthreads, 0, st, a, lines, vbits);
   TQ_LAUNCH_CHECK("batch_prep_kernel");
   for (int l = lines - 1; l >= 0; --l) {
     ba_run(vbits, a, l, p, st);
     TQ_LAUNCH_CHECK("batch_attn_kernel");
   }
-  hipLaunchKernelGGL(batch_join_kernel, dim3((unsigned)((qrows + 15) / 16)), dim3(64 * kJoinWaves), 0, st, a);
+  if (a.direct) {
+    const dim3 cut((unsigned)((a.line[0].waves - 1) * p.groups[0] + kTailBlocks));
+    if (p.prec) hipLaunchKernelGGL((batch_join_cut_kernel<true>), cut, dim3(64), 0, st, a);
+    else hipLaunchKernelGGL((batch_join_cut_kernel<false>), cut, dim3(64), 0, st, a);
+  } else {
+    hipLaunchKernelGGL(batch_join_kernel, dim3((unsigned)((qrows + 15) / 16)), dim3(64 * kJoinWaves), 0, st, a);
+  }
   TQ_LAUNCH_CHECK("batch_join_kernel");
   return TQ_OK;
 }

@@ -502,9 +502,7 @@ __global__ __launch_bounds__(64 * ba_waves(PREC, RW, NGR), ba_waves(PREC, RW, NG
         }
       }
       // wait states between the conversions and the products that read them
-      if constexpr (NGR == 3 && !PREC) {
-        mfma_operand_fence6(bh[0][0], bh[0][1], bh[1][0], bh[1][1], bh[2][0], bh[2][1]);
-      } else if constexpr (NGR == 2 && PREC) {
+      if constexpr (NGR == 2 && PREC) {
         mfma_operand_fence8(bh[0][0], bh[0][1], bh[1][0], bh[1][1], bl[0][0], bl[0][1], bl[1][0], bl[1][1]);
       } else {
 #pragma unroll
@@ -575,6 +573,23 @@ __global__ __launch_bounds__(64 * ba_waves(PREC, RW, NGR), ba_waves(PREC, RW, NG
       l[j] += __shfl_xor(l[j], 16, 64);
       l[j] += __shfl_xor(l[j], 32, 64);
       float f = vinv;
+      const bool done = NGR > 1 && whole && a.direct;
+      if constexpr (NGR > 1) {
+        if (done) {  // (sums over the weights' total: at most 2^14 in the norms' scale)
+          const float inv = l[j] == 0.f ? 0.f : 1.f / l[j];
+          ba_v4f x[4], out[4];
+#pragma unroll
+          for (int nb = 0; nb < 4; ++nb) x[nb] = o[j][nb] * inv;
+          ba_rotate_back<PREC>(a.vrot16, x, lane, out);
+          if (row0 + 16 * j + cr <= lastrow) {
+            int tok, qh;
+            place_of(j, tok, qh);
+#pragma unroll
+            for (int ob = 0; ob < 4; ++ob) ba_store(a, tok, qh, 16 * ob + 4 * g, out[ob] * vinv);
+            if (a.lse && g == 0) a.lse[(int64_t)tok * a.hq + qh] = ba_lse(m[j], l[j]);
+          }
+        }
+      }
       if constexpr (RW < 16) {
         float M = m[j];
 #pragma unroll
@@ -588,7 +603,7 @@ __global__ __launch_bounds__(64 * ba_waves(PREC, RW, NGR), ba_waves(PREC, RW, NG
       }
 #pragma unroll
       for (int nb = 0; nb < 4; ++nb) {
-        o[j][nb] *= f;
+        if (!done) o[j][nb] *= f;
         if constexpr (RW < 16) {
 #pragma unroll
           for (int x = RW; x < 16; x <<= 1)
@@ -596,7 +611,7 @@ __global__ __launch_bounds__(64 * ba_waves(PREC, RW, NGR), ba_waves(PREC, RW, NG
             for (int r = 0; r < 4; ++r) o[j][nb][r] += __shfl_xor(o[j][nb][r], x, 64);
         }
       }
-      if (cb == 0 && row0 + 16 * j + cr <= lastrow) {
+      if (!done && cb == 0 && row0 + 16 * j + cr <= lastrow) {
         int tok, qh;
         place_of(j, tok, qh);
         const int64_t rowid = (int64_t)tok * a.hq + qh;
@@ -616,7 +631,7 @@ __global__ __launch_bounds__(64 * ba_waves(PREC, RW, NGR), ba_waves(PREC, RW, NG
 
 template <int VB, bool SUB, bool PREC, bool WIDE>
 void ba_launch_kind(const BaArgs& a, int l, int rw, int groups, unsigned grid, hipStream_t st) {
-  constexpr int N = ba_groups(PREC);
+  constexpr int N = kBaGroups;
   const dim3 gr(grid), bl(64 * ba_waves(PREC, rw, groups));
   const BaLine& ln = a.line[l];
   if (groups > 1) hipLaunchKernelGGL((batch_attn_kernel<VB, SUB, PREC, 16, N, WIDE>), gr, bl, 0, st, a, ln);
