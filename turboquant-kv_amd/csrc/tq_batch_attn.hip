@@ -582,8 +582,9 @@ BaPlan ba_plan(tq_dtype q_dtype, int64_t n, int hq, int hkv, int64_t B, int64_t 
   for (int l = 0; l < (n_groups > 0 ? 2 : 1); ++l) {
     // A group of columns as wide as a segment's rows are on average: single tokens of few heads
     // use 4 or 8 of the 16 columns; rows beyond 16 share each tile's lookups.
-    // (whole tokens: a few rows of padding behind single tokens do not widen them)
-    const int64_t avg = std::max<int64_t>(1, n / std::max<int64_t>(l ? n_groups : B, 1)) * G;
+    // (rounded: a few rows of padding behind single tokens do not widen them)
+    const int64_t segs = std::max<int64_t>(l ? n_groups : B, 1);
+    const int64_t avg = std::max<int64_t>(1, (n + segs / 2) / segs) * G;
     p.rw[l] = avg <= 4 ? 4 : avg <= 8 ? 8 : 16;
     p.groups[l] = avg <= 16 ? 1 : kBaGroups;
     const int R = p.rw[l] * p.groups[l];

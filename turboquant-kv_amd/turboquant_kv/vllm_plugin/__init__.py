@@ -15,7 +15,9 @@ Paged operation (what vLLM's cache engine and scheduler provide, which the refer
 backend ignores): TurboQuantPagedKVCache.pools() holds K/V in block pools
 (vllm_plugin/paged.py), and TurboQuantAttentionImpl.forward with metadata that carries
 `block_tables` and `slot_mapping` stores the new tokens at their slots, runs causal
-prefill per prefill sequence and one paged decode launch for the decode sequences.
+prefill per prefill sequence and one paged decode launch for the decode sequences.  The
+Impl's alibi_slopes, sliding_window and logits_soft_cap, which the reference accepts and
+ignores (vllm_plugin:326-348), apply there (AttentionVariant).
 """
 
 from __future__ import annotations
@@ -28,7 +30,8 @@ import torch
 
 from turboquant_kv.cache import QuantizedKVCache
 from turboquant_kv.config import TurboQuantConfig
-from turboquant_kv.vllm_plugin.paged import PagedKVPools, TurboQuantAttentionMetadata
+from turboquant_kv.vllm_plugin.paged import (AttentionVariant, PagedKVPools,
+                                             TurboQuantAttentionMetadata)
 
 _VLLM_AVAILABLE = False
 try:  # pragma: no cover - vLLM is not installed in this image
@@ -185,6 +188,14 @@ def attention_step(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
     return out
 
 
+def attention_variant(alibi_slopes: Optional[List[float]] = None, sliding_window: Optional[int] = None,
+                      logits_soft_cap: Optional[float] = None) -> AttentionVariant:
+    """vLLM's attention arguments as an AttentionVariant (None, 0 and negative windows: off)."""
+    slopes = None if alibi_slopes is None else torch.as_tensor(alibi_slopes, dtype=torch.float32)
+    window = 0 if sliding_window is None or sliding_window < 0 else int(sliding_window)
+    return AttentionVariant(softcap=float(logits_soft_cap or 0.0), alibi_slopes=slopes, window=window)
+
+
 class TurboQuantAttentionImpl(AttentionImpl):
     """vLLM attention implementation over a TurboQuantPagedKVCache (vllm_plugin:312-412)."""
 
@@ -202,12 +213,14 @@ class TurboQuantAttentionImpl(AttentionImpl):
         self.alibi_slopes = alibi_slopes
         self.sliding_window = sliding_window
         self.logits_soft_cap = logits_soft_cap
+        self._variant = attention_variant(alibi_slopes, sliding_window, logits_soft_cap)
 
     def forward(self, query, key, value, kv_cache: TurboQuantPagedKVCache, attn_metadata,
                 k_scale: float = 1.0, v_scale: float = 1.0, attn_type: Any = None,
                 output: Optional[torch.Tensor] = None, **kwargs: Any) -> torch.Tensor:  # pragma: no cover
         if getattr(attn_metadata, "block_tables", None) is not None:
-            return kv_cache.pools().forward(query, key, value, attn_metadata, self.scale, output)
+            return kv_cache.pools().forward(query, key, value, attn_metadata, self.scale, output,
+                                            self._variant)
         layer_id: int = getattr(attn_metadata, "layer_id", 0)
         return attention_step(query, key, value, kv_cache, layer_id, self.scale, output)
 
@@ -257,11 +270,12 @@ def register() -> None:
 
 def paged_attention_step(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
                          kv_cache: TurboQuantPagedKVCache, metadata: TurboQuantAttentionMetadata,
-                         scale: float, output: Optional[torch.Tensor] = None) -> torch.Tensor:
+                         scale: float, output: Optional[torch.Tensor] = None,
+                         variant: Optional[AttentionVariant] = None) -> torch.Tensor:
     """TurboQuantAttentionImpl.forward on paged metadata, callable without vLLM."""
-    return kv_cache.pools().forward(query, key, value, metadata, scale, output)
+    return kv_cache.pools().forward(query, key, value, metadata, scale, output, variant)
 
 
 __all__ = ["TurboQuantKVCacheConfig", "TurboQuantPagedKVCache", "TurboQuantAttentionBackend",
-           "TurboQuantAttentionImpl", "TurboQuantAttentionMetadata", "PagedKVPools",
+           "TurboQuantAttentionImpl", "TurboQuantAttentionMetadata", "PagedKVPools", "AttentionVariant", "attention_variant",
            "attention_step", "paged_attention_step", "register"]

@@ -25,6 +25,14 @@ power of two >= 16) keeps the quantized layers in the decode layout instead: key
 sub-blocks) below -- read by the MFMA decode kernel through the block tables
 (`decode_attention_paged_dl`); a prefill sequence runs the causal prefill kernel over the
 same pools (`prefill_attention_paged_dl`).
+
+Steps that those two do not express -- capped or biased scores, windows, prefix and document
+masks (AttentionVariant and the metadata's optional fields), shared prefixes, or lengths that
+only the device knows (`ragged`) -- run the ragged batch operator over decode-layout pools
+(`attention_batch_paged_dl`, `attention_shared_prefix_paged_dl`); over the other layouts
+the same scores are formed per sequence from the packed rows.  TurboQuantAttentionMetadata.
+from_lengths makes a ragged step's metadata on the device (`paged_batch_plan`,
+`shared_prefix_groups`).
 """
 
 from __future__ import annotations
@@ -65,6 +73,51 @@ class TurboQuantAttentionMetadata:
     layer_id: int = 0
     query_start_loc_cpu: Optional[List[int]] = None
     seq_lens_cpu: Optional[List[int]] = None
+    # masks: the positions each token sees (prefix_lens [num_seqs]: all tokens of a sequence see
+    # its first prefix_lens; token_starts [num_tokens]: the first position each token sees)
+    prefix_lens: Optional[torch.Tensor] = None
+    token_starts: Optional[torch.Tensor] = None
+    # sequences group_start_loc[g] .. group_start_loc[g + 1] - 1 share their first
+    # shared_lens[g] tokens' blocks, which are read once for all of them
+    group_start_loc: Optional[torch.Tensor] = None
+    shared_lens: Optional[torch.Tensor] = None
+    # any mix of prompts, chunks and single tokens in any order, num_prefills not used
+    ragged: bool = False
+
+    @classmethod
+    def from_lengths(cls, new_lens: torch.Tensor, context_lens: torch.Tensor,
+                     block_tables: torch.Tensor, free_blocks: torch.Tensor, block_size: int,
+                     num_tokens: int, free_start: Optional[torch.Tensor] = None,
+                     min_shared_tokens: int = 0, layer_id: int = 0):
+        """A ragged step's metadata from the requests' lengths, made on the device: request r
+        holds context_lens[r] tokens and brings new_lens[r] more, whose blocks come from
+        free_blocks and are written into block_tables (ops.paged_batch_plan).  With
+        min_shared_tokens > 0, neighbouring requests whose tables begin with the same blocks for
+        that many tokens or more are taken together (ops.shared_prefix_groups).
+        -> (metadata, positions [num_tokens], blocks_used [1])."""
+        qsl, lens, slots, pos, _, used = ops.paged_batch_plan(
+            new_lens, context_lens, block_tables, free_blocks, block_size, num_tokens, free_start)
+        groups = shared = None
+        if min_shared_tokens > 0:
+            groups, shared = ops.shared_prefix_groups(block_tables, context_lens, block_size,
+                                                      min_shared_tokens)
+        md = cls(slots, lens, block_tables, qsl, 0, layer_id, group_start_loc=groups,
+                 shared_lens=shared, ragged=True)
+        return md, pos, used
+
+
+@dataclass
+class AttentionVariant:
+    """How a layer's scores are changed before the softmax: scaled, capped (softcap *
+    tanh(score / softcap); 0: not), biased (alibi_slopes [Hq] * (key position - query
+    position)), and kept to the last `window` positions, the query's own included (0: all)."""
+
+    softcap: float = 0.0
+    alibi_slopes: Optional[torch.Tensor] = None
+    window: int = 0
+
+    def __bool__(self) -> bool:
+        return self.softcap > 0 or self.alibi_slopes is not None or self.window > 0
 
 
 def _shares_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -330,14 +383,99 @@ class PagedKVPools:
                                              seq_lens, self.kcen, self.vcen, self.R_k, self.R_v,
                                              float(scale))
 
+    def attend(self, layer: int, q: torch.Tensor, md: TurboQuantAttentionMetadata, scale: float,
+               variant: Optional[AttentionVariant] = None,
+               output: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Attention of a batch's tokens q [num_tokens, Hq, d] over their sequences as stored,
+        with a layer's score variant and the metadata's masks and shared prefixes, in any mix of
+        lengths -> [num_tokens, Hq, d] in q's dtype (zeros behind the last sequence; a given
+        output keeps its rows there).  Decode-layout pools: one call, no host copy of lengths."""
+        v = variant if variant is not None else AttentionVariant()
+        st = self.layers[layer]
+        q = q.to(self.device)
+        if v.alibi_slopes is not None and not v.alibi_slopes.is_cuda:
+            v.alibi_slopes = v.alibi_slopes.to(self.device)  # once: later steps may be captured
+        kw = dict(softcap=v.softcap, alibi_slopes=v.alibi_slopes, window=v.window,
+                  prefix_lens=md.prefix_lens, token_starts=md.token_starts)
+        if "kp" in st:
+            wide = q.dtype == torch.float64  # computed in float32, as the other paths do
+            qc = q.float() if wide else q
+            # the kernels read q while they write: a result in its memory takes a copy
+            direct = (output is not None and output.device == q.device and output.shape == q.shape
+                      and output.dtype == qc.dtype and not _shares_memory(output, q)
+                      and output.stride()[1:] == (q.shape[2], 1) and output.data_ptr() % 16 == 0
+                      and output.stride(0) >= q.shape[1] * q.shape[2]
+                      and output.stride(0) * output.element_size() % 16 == 0)
+            args = [qc, st["kp"], st["kn"], st["vt"], st["vn"], md.block_tables, md.query_start_loc,
+                    md.seq_lens]
+            tail = [self.kcen, self.vcen, self.R_k, self.R_v, float(scale)]
+            if direct:
+                kw["out"] = output
+            if md.group_start_loc is not None:
+                args += [md.group_start_loc, md.shared_lens]
+                res = ops.attention_shared_prefix_paged_dl(*args, *tail, **kw)
+            else:
+                res = ops.attention_batch_paged_dl(*args, *tail, **kw)
+            if output is None or direct:
+                return res.to(q.dtype) if output is None else res
+            # a few rows behind the last sequence keep the output's values
+            live = torch.arange(q.shape[0], device=q.device) < md.query_start_loc.to(q.device)[-1]
+            output.copy_(torch.where(live[:, None, None], res.to(output.dtype), output))
+            return output
+        out = output if output is not None else torch.zeros_like(q)
+        qsl = md.query_start_loc_cpu or md.query_start_loc.tolist()
+        lens = md.seq_lens_cpu or md.seq_lens.tolist()
+        for b, T in enumerate(lens):
+            i, j = qsl[b], qsl[b + 1]
+            if j > i:
+                out[i:j] = self._attend_rows(
+                    layer, q[i:j], md.block_tables[b], int(T), scale, v,
+                    None if md.prefix_lens is None else int(md.prefix_lens[b]),
+                    None if md.token_starts is None else md.token_starts[i:j]).to(out.dtype)
+        return out
+
+    def _attend_rows(self, layer, q, block_table, T, scale, v, prefix, starts):
+        """attend() of one sequence's rows over a bit-plane, prod or unquantized layer."""
+        n, Hq, d = q.shape
+        H, dev = self.num_kv_heads, self.device
+        G = Hq // H
+        out = torch.zeros(n, Hq, d, dtype=torch.float32, device=dev)
+        if T <= 0:
+            return out
+        keys, vals = self.sequence_kv(layer, block_table, T)
+        pos = torch.arange(T - n, T, device=dev)[:, None]
+        j = torch.arange(T, device=dev)[None, :]
+        seen = (j <= pos) if prefix is None else (j <= pos) | (j < prefix)
+        if v.window > 0:
+            seen &= j > pos - v.window
+        if starts is not None:
+            seen &= j >= starts.to(dev)[:, None]
+        qf = q.float()
+        for g in range(H):
+            s = (qf[:, g * G:(g + 1) * G].transpose(0, 1).reshape(G * n, d) @ keys[g].t()).view(G, n, T) * scale
+            if v.softcap > 0:
+                s = v.softcap * torch.tanh(s / v.softcap)
+            if v.alibi_slopes is not None:
+                s = s + v.alibi_slopes.to(dev, torch.float32)[g * G:(g + 1) * G, None, None] * (j - pos)
+            s = s.masked_fill(~seen, float("-inf"))
+            w = torch.softmax(s, -1).masked_fill(~seen.any(-1)[:, None], 0.0)
+            o = w.reshape(G * n, T) @ vals[g]
+            out[:, g * G:(g + 1) * G] = o.view(G, n, d).transpose(0, 1)
+        return out
+
     def forward(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
                 md: TurboQuantAttentionMetadata, scale: float,
-                output: Optional[torch.Tensor] = None) -> torch.Tensor:
+                output: Optional[torch.Tensor] = None,
+                variant: Optional[AttentionVariant] = None) -> torch.Tensor:
         """vLLM attention step: store the batch's new K/V at their slots, then causal
-        prefill for the leading sequences and one fused decode launch for the rest.
+        prefill for the leading sequences and one fused decode launch for the rest; a score
+        variant, masks, shared prefixes or ragged metadata: attend() for all of them.
         query [num_tokens, Hq, d], key/value [num_tokens, Hkv, d]."""
         layer = md.layer_id
         self.write(layer, key, value, md.slot_mapping)
+        if (variant or md.ragged or md.prefix_lens is not None or md.token_starts is not None
+                or md.group_start_loc is not None):
+            return self.attend(layer, query, md, scale, variant, output)
         npf = md.num_prefills
         if (npf == 0 and output is None and 0 < query.shape[0] == md.block_tables.shape[0]
                 and query.is_contiguous()):
