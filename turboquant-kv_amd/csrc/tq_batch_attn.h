@@ -52,6 +52,7 @@ namespace tq {
 // sequences of up to 32k tokens, 4-bit values, 128 -> 117 us; bf16: 89 and 91 us.
 constexpr int ba_waves(bool prec, int rw, int groups) { return prec && groups == 1 && rw < 16 ? 12 : 8; }
 constexpr int kBaMaxSegs = 8191;  // sequences or groups of a call: the preparing kernel's LDS
+constexpr int kBaQueryTop = 14;   // rotated queries are scaled to at most 2^14 (fp16's range ends at 2^16)
 constexpr int kBaOver = 3;        // an (item, head)'s cost besides its tiles, in tiles
 constexpr int kBaGroups = 2;      // groups of 16 rows a wave takes where rows abound: three spill
 // Floats of a partial slot of R rows: sums [R][64], (maximum, sum) [R][2].
@@ -131,7 +132,7 @@ struct BaArgs {
   // made by the preparing kernel
   _Float16* qhi;               // [n_tokens * hq][64] rotated queries over a power of two: hi,
   _Float16* qlo;               // and lo parts (fp32 / fp16 queries)
-  float* qscale_inv;           // [n_tokens * hq] what undoes it and the key centroids' scale
+  int32_t* qexp;               // [n_tokens * hq] log2 of what undoes it and the key centroids' scale
   BaEntry* entries;            // [256]
   _Float16* vrot16;            // R_v's operands, [2 parts][4 ob][2 s][64 lanes][8]: see ba_rotate_back
   int direct;                  // (no groups) waves write the results of whole items of many rows

@@ -118,14 +118,16 @@ __device__ __forceinline__ void ba_lay_out(const BaArgs& a, int32_t* base_s, int
       it.table = x.table;
       it.lo = x.lo;
       it.hi = x.hi;
-      // Document starts bound single tokens; the waves of longer items skip the tiles that all
-      // their own rows' starts leave out.
       int64_t lo = x.lo, hi = x.hi;
       if (L == 0) {
         const int i0t = (int)ba_div(row0, a.G), i1t = min(x.ntok - 1, (int)ba_div(row0 + R - 1, a.G));
         hi = min<int64_t>(hi, max<int64_t>((int64_t)x.past + i1t + 1, x.prefix));
         if (a.window > 0) lo = max<int64_t>(lo, (int64_t)x.past + i0t + 1 - a.window);
-        if (a.token_starts && x.ntok == 1 && hi > 0) lo = max<int64_t>(lo, a.token_starts[x.tok0]);
+        if (a.token_starts && hi > lo) {
+          int first = INT_MAX;
+          for (int t = i0t; t <= i1t; ++t) first = min(first, a.token_starts[x.tok0 + t]);
+          lo = max<int64_t>(lo, first);
+        }
       }
       it.t0 = hi > lo ? (int)(lo >> 6) : 0;
       it.nt = hi > lo ? (int)((hi + 63) >> 6) - it.t0 : 0;
@@ -239,7 +241,7 @@ __device__ __forceinline__ void ba_find_token(const BaArgs& a, int t) {
 
 // Workgroups 0 .. n_lines - 1 lay the lines out, the next makes the tables, the others rotate
 // 16 rows (a token's head each) a wave and round: Qrot = q R_k^T qscale, scaled by a power of
-// two into [0.5, 1) and split into fp16 hi (and lo) parts.  Lane (c, g) ends with dims 16 g ..
+// two into [2^(kBaQueryTop - 1), 2^kBaQueryTop) and split into fp16 hi (and lo) parts.  Lane (c, g) ends with dims 16 g ..
 // 16 g + 15 of row c, the order in which its key bytes come: output 4 k + r of product mb is
 // dim 16 k + 4 mb + r.
 //   float32 queries: v_mfma_f32_16x16x4f32, 64 products of 8 passes a round.
@@ -325,7 +327,7 @@ __device__ __forceinline__ void ba_rotate_rows(const BaArgs& a, int64_t blk, int
     qm = fmaxf(qm, __shfl_xor(qm, 16, 64));
     qm = fmaxf(qm, __shfl_xor(qm, 32, 64));
     const int e = ba_exponent(qm);
-    const float qsc = ldexpf(1.f, -e);
+    const float qsc = ldexpf(1.f, kBaQueryTop - e);
     ba_v8h hi[2], lo[2];
 #pragma unroll
     for (int s = 0; s < 2; ++s)
@@ -341,7 +343,7 @@ __device__ __forceinline__ void ba_rotate_rows(const BaArgs& a, int64_t blk, int
         *reinterpret_cast<ba_v8h*>(a.qhi + row * 64 + 16 * g + 8 * s) = hi[s];
         if constexpr (DT != TQ_BF16) *reinterpret_cast<ba_v8h*>(a.qlo + row * 64 + 16 * g + 8 * s) = lo[s];
       }
-      if (g == 0) a.qscale_inv[row] = ldexpf(1.f, e + ke);
+      if (g == 0) a.qexp[row] = qm > 0.f ? e - kBaQueryTop + ke : -1000;  // (zeros scale no other row)
     }
   }
 }
@@ -608,7 +610,7 @@ size_t ba_place(const BaPlan& p, int64_t n, int hq, char* at, BaArgs* a) {
   BaArgs b{};
   b.entries = reinterpret_cast<BaEntry*>(take(256 * sizeof(BaEntry)));
   b.tokens = reinterpret_cast<BaToken*>(take(n * sizeof(BaToken)));
-  b.qscale_inv = reinterpret_cast<float*>(take(rows * 4));
+  b.qexp = reinterpret_cast<int32_t*>(take(rows * 4));
   b.qhi = reinterpret_cast<_Float16*>(take(rows * 128));
   b.vrot16 = reinterpret_cast<_Float16*>(take(2 * 4096 * sizeof(_Float16)));
   if (p.prec) b.qlo = reinterpret_cast<_Float16*>(take(rows * 128));
@@ -627,7 +629,7 @@ size_t ba_place(const BaPlan& p, int64_t n, int hq, char* at, BaArgs* a) {
     ln.row_stats = reinterpret_cast<float*>(take(rows * 8));
   }
   if (a) {
-    a->entries = b.entries; a->vrot16 = b.vrot16; a->tokens = b.tokens; a->qscale_inv = b.qscale_inv; a->qhi = b.qhi; a->qlo = b.qlo;
+    a->entries = b.entries; a->vrot16 = b.vrot16; a->tokens = b.tokens; a->qexp = b.qexp; a->qhi = b.qhi; a->qlo = b.qlo;
     a->line[0] = b.line[0]; a->line[1] = b.line[1];
   }
   return used;

@@ -15,24 +15,22 @@ __device__ __forceinline__ ba_v8h ba_h8(uint32_t a, uint32_t b, uint32_t c, uint
   return __builtin_bit_cast(ba_v8h, t);
 }
 
-// cap2 tanh(y / cap2).  tanh z = 1 - 2 / (1 + e^(2 z)), exact at both ends (the exponential
-// overflows to inf or vanishes); its absolute error of about 2^-23 is cap2 2^-23 in the score.
-// EXACT: below |z| = 0.3 the odd series instead (the next term is 6e-10 relative), whose error
-// is relative.
+// cap2 tanh(z) of x = 2 z log2(e).  tanh z = 1 - 2 / (1 + e^(2 z)), exact at both ends (the
+// exponential overflows to inf or vanishes); its absolute error of about 2^-23 is cap2 2^-23 in
+// the score.  EXACT: below |z| = 0.3 the odd series instead (the next term is 6e-10 relative),
+// whose error is relative.
 template <bool EXACT>
-__device__ __forceinline__ float ba_softcap(float y, float cap2, float cap2_inv) {
-  const float z = y * cap2_inv;
-  const float e = __builtin_amdgcn_exp2f(z * 2.885390081777927f);
-  const float big = fmaf(-2.f * cap2, __builtin_amdgcn_rcpf(1.f + e), cap2);
+__device__ __forceinline__ float ba_softcap(float x, float cap2) {
+  const float big = fmaf(-2.f * cap2, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x)), cap2);
   if constexpr (!EXACT) {
     return big;
   } else {
-    const float w = z * z;
+    const float z = x * 0.34657359027997264f, w = z * z;
     float p = fmaf(w, -0.00886323552990f, 0.0218694885361f);
     p = fmaf(w, p, -0.0539682539683f);
     p = fmaf(w, p, 0.133333333333f);
     p = fmaf(w, p, -0.333333333333f);
-    const float small = fmaf(y * w, p, y);
+    const float y = z * cap2, small = fmaf(y * w, p, y);
     return w < 0.09f ? small : big;
   }
 }
@@ -52,6 +50,24 @@ __device__ __forceinline__ T ba_load(__amdgpu_buffer_rsrc_t rs, uint32_t lane_of
   if constexpr (sizeof(T) == 4) return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(rs, lane_off, off, 0));
   else if constexpr (sizeof(T) == 8) return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b64(rs, lane_off, off, 0));
   else return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b128(rs, lane_off, off, 0));
+}
+
+// fp16 products a u (low half) and b v, each rounded once.
+__device__ __forceinline__ uint32_t ba_products(float a, float u, float b, float v) {
+  uint32_t r;
+  asm("v_fma_mixlo_f16 %0, %1, %2, 0\n\tv_fma_mixhi_f16 %0, %3, %4, 0" : "=&v"(r) : "v"(a), "v"(u), "v"(b), "v"(v));
+  return r;
+}
+
+// fp16 hi and lo parts of a (low half) and b.  (Each is pinned as one fp32 value first: a product
+// folded into both conversions would be rounded apart.)
+__device__ __forceinline__ void ba_split(float a, float b, uint32_t& hi, uint32_t& lo) {
+  typedef float v2f __attribute__((ext_vector_type(2)));
+  typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+  asm("" : "+v"(a), "+v"(b));
+  const v2h h = __builtin_convertvector((v2f){a, b}, v2h);
+  hi = __builtin_bit_cast(uint32_t, h);
+  lo = __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f){a - (float)h[0], b - (float)h[1]}, v2h));
 }
 
 // The larger of two numbers in one instruction (fmaxf first quiets operands it cannot see
@@ -139,7 +155,6 @@ __global__ __launch_bounds__(64 * ba_waves(PREC, RW, NGR), ba_waves(PREC, RW, NG
   float* const snorm = reinterpret_cast<float*>(smem + kBaNorms) + wave * 128;
   const __amdgpu_buffer_rsrc_t krs = buf_rsrc(a.kpairs, 0xFFFFFFFFu), vrs = buf_rsrc(a.vtiles, 0xFFFFFFFFu);
   const __amdgpu_buffer_rsrc_t knrs = buf_rsrc(a.knorms, 0xFFFFFFFFu), vnrs = buf_rsrc(a.vnorms, 0xFFFFFFFFu);
-  const bool mods = a.cap2 != 0.f || a.slopes != nullptr;
   int64_t pos = (int64_t)w * chunk;
   const int64_t end = min(pos + chunk, total);
 
@@ -170,7 +185,8 @@ __global__ __launch_bounds__(64 * ba_waves(PREC, RW, NGR), ba_waves(PREC, RW, NG
     };
     // ---- rows: group j's column c holds row row0 + 16 j + cr (past the end: the last)
     int lo[NGR], hi[NGR], qpos[NGR];
-    float slope[NGR], kinv[NGR];
+    float slope[NGR];
+    int qe[NGR], qtop = INT_MIN;
     ba_v8h qhi[NGR][2], qlo[PREC ? NGR : 1][2];
 #pragma unroll
     for (int j = 0; j < NGR; ++j) {
@@ -181,7 +197,8 @@ __global__ __launch_bounds__(64 * ba_waves(PREC, RW, NGR), ba_waves(PREC, RW, NG
       hi[j] = min(t.hi, it_hi);
       qpos[j] = t.pos;
       const int64_t rowid = (int64_t)tok * a.hq + qh;
-      kinv[j] = a.qscale_inv[rowid];
+      qe[j] = a.qexp[rowid];
+      qtop = max(qtop, qe[j]);
       slope[j] = a.slopes ? a.slopes[qh] * 1.4426950408889634f : 0.f;
 #pragma unroll
       for (int s = 0; s < 2; ++s) {  // dims 16 g + 8 s ..
@@ -189,6 +206,24 @@ __global__ __launch_bounds__(64 * ba_waves(PREC, RW, NGR), ba_waves(PREC, RW, NG
         if constexpr (PREC) qlo[j][s] = *reinterpret_cast<const ba_v8h*>(a.qlo + rowid * 64 + 16 * g + 8 * s);
       }
     }
+    // One power of two for all the wave's rows, so that it goes with the key norms: shorter queries
+    // are scaled down to the longest's.  Errors stay under 2^-22 (bf16 queries: 2^-11) of a row's
+    // own length down to lengths 2^-17 (2^-28) of the longest row's.
+    qtop = ba_wave_max(qtop);
+#pragma unroll
+    for (int j = 0; j < NGR; ++j)
+      if (__any(qe[j] != qtop)) {
+        const float f = __builtin_amdgcn_ldexpf(1.f, max(qe[j] - qtop, -100));
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            qhi[j][s][i] = (_Float16)((float)qhi[j][s][i] * f);
+            if constexpr (PREC) qlo[j][s][i] = (_Float16)((float)qlo[j][s][i] * f);
+          }
+      }
+    // the key norms' factor: scores in the log2 domain, or what ba_softcap takes
+    const float kscale = __builtin_amdgcn_ldexpf(a.cap2 != 0.f ? 2.885390081777927f * a.cap2_inv : 1.f, qtop);
     int lo_min = INT_MAX, lo_max = 0, hi_min = INT_MAX, hi_max = 0;
 #pragma unroll
     for (int j = 0; j < NGR; ++j) {
@@ -201,13 +236,7 @@ __global__ __launch_bounds__(64 * ba_waves(PREC, RW, NGR), ba_waves(PREC, RW, NG
     lo_max = ba_wave_max(lo_max);
     hi_min = ba_wave_min(hi_min);
     hi_max = ba_wave_max(hi_max);
-    // tiles of the piece; document starts may leave out some that the line holds
-    int k0 = t0 + ta, nw = tb - ta;
-    if (a.token_starts) {
-      const int k1 = hi_max > lo_min ? min(k0 + nw, (int)(((int64_t)hi_max + 63) >> 6)) : k0;
-      k0 = max(k0, lo_min >> 6);
-      nw = max(0, k1 - k0);
-    }
+    const int k0 = t0 + ta, nw = tb - ta;  // tiles of the piece
 
     float m[NGR], l[NGR];
     ba_v4f o[NGR][4];
@@ -327,7 +356,7 @@ __global__ __launch_bounds__(64 * ba_waves(PREC, RW, NGR), ba_waves(PREC, RW, NG
 #pragma unroll
           for (int nb = 0; nb < 4; ++nb) o[j][nb] *= f;
       }
-      snorm[lane] = t.nk;
+      snorm[lane] = t.nk * kscale;
       snorm[64 + lane] = nvl * vs.s;
       __builtin_amdgcn_wave_barrier();
 
@@ -355,8 +384,7 @@ __global__ __launch_bounds__(64 * ba_waves(PREC, RW, NGR), ba_waves(PREC, RW, NG
       };
 
 
-      // ---- scores over the norm's and the scales' powers of two: entry k of a lane is its copy's
-      // 16-token group NB cb + k
+      // ---- scores: entry k of a lane is its copy's 16-token group NB cb + k
       ba_v4f sv[NGR][NB], all[NGR][4];
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
@@ -407,18 +435,22 @@ __global__ __launch_bounds__(64 * ba_waves(PREC, RW, NGR), ba_waves(PREC, RW, NG
 #pragma unroll
           for (int r = 0; r < 4; ++r) sv[j][k][r] *= nk4[r];
       }
-      if (mods) {  // to the log2 domain, capped and biased
+      if (a.cap2 != 0.f) {
+#pragma unroll
+        for (int j = 0; j < NGR; ++j)
+#pragma unroll
+          for (int k = 0; k < NB; ++k)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sv[j][k][r] = ba_softcap<PREC>(sv[j][k][r], a.cap2);
+      }
+      if (a.slopes) {
 #pragma unroll
         for (int j = 0; j < NGR; ++j) {
           const float d0 = (float)(p0 + tg - qpos[j]);
 #pragma unroll
           for (int k = 0; k < NB; ++k)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              float y = sv[j][k][r] * kinv[j];
-              if (a.cap2 != 0.f) y = ba_softcap<PREC>(y, a.cap2, a.cap2_inv);
-              sv[j][k][r] = fmaf(slope[j], d0 + (float)(16 * k + r), y);
-            }
+            for (int r = 0; r < 4; ++r) sv[j][k][r] = fmaf(slope[j], d0 + (float)(16 * k + r), sv[j][k][r]);
         }
       }
       if (mask) {
@@ -446,8 +478,7 @@ __global__ __launch_bounds__(64 * ba_waves(PREC, RW, NGR), ba_waves(PREC, RW, NG
 #pragma unroll
           for (int r = 0; r < 4; ++r) mx = fmaxf(mx, sv[j][k][r]);
         mx = ba_max4(mx);
-        const float kin = mods ? 1.f : kinv[j];
-        const float mn = fmaxf(m[j], mx * kin);
+        const float mn = fmaxf(m[j], mx);
         const float ms = mn == -INFINITY ? 0.f : mn;
         if (__any(mn != m[j])) {
           const float alpha = __builtin_amdgcn_exp2f(m[j] - ms);
@@ -456,49 +487,44 @@ __global__ __launch_bounds__(64 * ba_waves(PREC, RW, NGR), ba_waves(PREC, RW, NG
           for (int nb = 0; nb < 4; ++nb) o[j][nb] *= alpha;
         }
         m[j] = mn;
-        typedef _Float16 v4h __attribute__((ext_vector_type(4)));
-        v4h ph[NB], pl[NB];
+        // weights times value norms, two fp16 a word: word q of group k holds tokens 2 q, 2 q + 1
+        uint32_t ph[NB][2], pl[PREC ? NB : 1][2];
 #pragma unroll
         for (int k = 0; k < NB; ++k)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
+          for (int q = 0; q < 2; ++q) {
             // results below 2^-126 flush to 0: nothing beside the running maximum's 1
-            const float p = __builtin_amdgcn_exp2f(fmaf(sv[j][k][r], kin, -ms));
-            l[j] += p;
-            const float v = p * nv4[k][r];
-            if constexpr (PREC) {
-              _Float16 hv, lv;
-              split_f16(v, hv, lv);
-              ph[k][r] = hv;
-              pl[k][r] = lv;
-            } else {
-              ph[k][r] = (_Float16)v;
-            }
+            const float pa = __builtin_amdgcn_exp2f(sv[j][k][2 * q] - ms);
+            const float pb = __builtin_amdgcn_exp2f(sv[j][k][2 * q + 1] - ms);
+            l[j] += pa + pb;
+            if constexpr (PREC) ba_split(pa * nv4[k][2 * q], pb * nv4[k][2 * q + 1], ph[k][q], pl[k][q]);
+            else ph[k][q] = ba_products(pa, nv4[k][2 * q], pb, nv4[k][2 * q + 1]);
           }
         if (__builtin_expect(odd, 0)) {  // rows that do not see it must not take 0 * inf
           asm volatile("");
 #pragma unroll
           for (int k = 0; k < NB; ++k)
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (sv[j][k][r] == -INFINITY) {
-                ph[k][r] = (_Float16)0.f;
-                if constexpr (PREC) pl[k][r] = (_Float16)0.f;
-              }
+            for (int q = 0; q < 2; ++q) {
+              const uint32_t keep = (sv[j][k][2 * q] == -INFINITY ? 0u : 0xFFFFu) |
+                                    (sv[j][k][2 * q + 1] == -INFINITY ? 0u : 0xFFFF0000u);
+              ph[k][q] &= keep;
+              if constexpr (PREC) pl[k][q] &= keep;
+            }
         }
         // the second products' operand: 16-token group b in half b % 2 of part b / 2
-        const v4h zero = {(_Float16)0.f, (_Float16)0.f, (_Float16)0.f, (_Float16)0.f};
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          const bool mine = RW == 16 || cb == b / NB;
-          const v4h x = mine ? ph[b % NB] : zero;
+        for (int s = 0; s < 2; ++s) {
+          uint32_t x[4], y[4];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) bh[j][b >> 1][4 * (b & 1) + r] = x[r];
-          if constexpr (PREC) {
-            const v4h y = mine ? pl[b % NB] : zero;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) bl[j][b >> 1][4 * (b & 1) + r] = y[r];
+          for (int q = 0; q < 4; ++q) {
+            const int b = 2 * s + (q >> 1);
+            const bool mine = RW == 16 || cb == b / NB;
+            x[q] = mine ? ph[b % NB][q & 1] : 0u;
+            if constexpr (PREC) y[q] = mine ? pl[b % NB][q & 1] : 0u;
           }
+          bh[j][s] = ba_h8(x[0], x[1], x[2], x[3]);
+          if constexpr (PREC) bl[j][s] = ba_h8(y[0], y[1], y[2], y[3]);
         }
       }
       // wait states between the conversions and the products that read them
