@@ -50,7 +50,9 @@ namespace tq {
 // Waves of a workgroup (one per CU: the tables fill its LDS).  Single tokens of fp32 / fp16
 // queries: 12 (168 registers a wave) instead of 8 hide more of the three products' latency: 48
 // sequences of up to 32k tokens, 4-bit values, 128 -> 117 us; bf16: 89 and 91 us.
-constexpr int ba_waves(bool prec, int rw, int groups) { return prec && groups == 1 && rw < 16 ? 12 : 8; }
+constexpr int ba_waves(bool prec, int rw, int groups, bool pair) {
+  return prec && groups == 1 && rw < 16 && !pair ? 12 : 8;
+}
 constexpr int kBaMaxSegs = 8191;  // sequences or groups of a call: the preparing kernel's LDS
 constexpr int kBaQueryTop = 14;   // rotated queries are scaled to at most 2^14 (fp16's range ends at 2^16)
 constexpr int kBaOver = 3;        // an (item, head)'s cost besides its tiles, in tiles
@@ -145,12 +147,12 @@ typedef _Float16 ba_v8h __attribute__((ext_vector_type(8)));
 typedef uint32_t ba_u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t ba_u32x2 __attribute__((ext_vector_type(2)));
 
-// Launches the main kernel of value width VB over line `l` (rw: 4, 8 or 16 rows a group of
-// columns; SUB: pools of 16-token value sub-blocks; wide: pools of 4 GB and more).
+// Launches the main kernel of value width VB over line 0, or (pair) both lines (rw: 4, 8 or 16 rows
+// a group of columns; SUB: pools of 16-token value sub-blocks; wide: pools of 4 GB and more).
 template <int VB, bool SUB>
-void ba_launch(const BaArgs& a, int l, bool wide, bool prec, int rw, int groups, unsigned grid, hipStream_t st);
+void ba_launch(const BaArgs& a, bool pair, bool wide, bool prec, int rw, int groups, unsigned grid, hipStream_t st);
 #define BA_LAUNCH(VB, SUB) \
-  template void ba_launch<VB, SUB>(const BaArgs&, int, bool, bool, int, int, unsigned, hipStream_t);
+  template void ba_launch<VB, SUB>(const BaArgs&, bool, bool, bool, int, int, unsigned, hipStream_t);
 extern BA_LAUNCH(2, false) extern BA_LAUNCH(2, true)
 extern BA_LAUNCH(3, false) extern BA_LAUNCH(3, true)
 extern BA_LAUNCH(4, false) extern BA_LAUNCH(4, true)

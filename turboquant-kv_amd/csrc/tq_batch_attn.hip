@@ -249,12 +249,29 @@ __device__ __forceinline__ void ba_find_token(const BaArgs& a, int t) {
 //   the rounds, in three bfloat16 or two float16 parts (times 2^10: none is subnormal), which
 //   carry 24 and 22 bits: 24 or 16 products of 4 passes.
 template <int DT>
-__device__ __forceinline__ void ba_rotate_rows(const BaArgs& a, int64_t blk, int64_t n_blks) {
+__device__ __forceinline__ void ba_rotate_rows(const BaArgs& a, int64_t blk, int64_t n_blks, float* rk_s) {
 #pragma clang fp contract(off)
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int c = lane & 15, g = lane >> 4;
   const int64_t n_rows = (int64_t)a.n_tokens * a.hq;
+  // R_k through LDS, [64][68]: read along its memory whichever its order, used by rows
+  {
+    const int at = 8 * tid;
+    const ba_v4f x0 = *reinterpret_cast<const ba_v4f*>(a.krot + at), x1 = *reinterpret_cast<const ba_v4f*>(a.krot + at + 4);
+    const int along = at & 63, across = at >> 6;
+    if (a.krot_col == 1) {
+      *reinterpret_cast<ba_v4f*>(rk_s + across * 68 + along) = x0;
+      *reinterpret_cast<ba_v4f*>(rk_s + across * 68 + along + 4) = x1;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        rk_s[(along + i) * 68 + across] = x0[i];
+        rk_s[(along + 4 + i) * 68 + across] = x1[i];
+      }
+    }
+  }
   const int ke = ba_exponent(wave_max(lane < 16 ? fabsf(a.kcen[lane]) : 0.f));
+  __syncthreads();
   constexpr int PARTS = DT == TQ_BF16 ? 3 : 2;
   typedef __bf16 v8b __attribute__((ext_vector_type(8)));
   using v8 = std::conditional_t<DT == TQ_BF16, v8b, ba_v8h>;
@@ -268,7 +285,7 @@ __device__ __forceinline__ void ba_rotate_rows(const BaArgs& a, int64_t blk, int
       for (int s = 0; s < 2; ++s)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          float v = kUp * a.krot[(16 * (c >> 2) + 4 * mb + (c & 3)) * a.krot_row + (32 * s + 8 * g + i) * a.krot_col];
+          float v = kUp * rk_s[(16 * (c >> 2) + 4 * mb + (c & 3)) * 68 + 32 * s + 8 * g + i];
 #pragma unroll
           for (int p = 0; p < PARTS; ++p) {
             const elem x = (elem)v;
@@ -294,7 +311,7 @@ __device__ __forceinline__ void ba_rotate_rows(const BaArgs& a, int64_t blk, int
         float rk[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          rk[i] = a.krot[(16 * (c >> 2) + 4 * mb + (c & 3)) * a.krot_row + (16 * g + i) * a.krot_col];
+          rk[i] = rk_s[(16 * (c >> 2) + 4 * mb + (c & 3)) * 68 + 16 * g + i];
         d[mb] = (ba_v4f){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < 16; ++i) d[mb] = __builtin_amdgcn_mfma_f32_16x16x4f32(rk[i], qv[i], d[mb], 0, 0, 0);
@@ -353,6 +370,7 @@ __global__ __launch_bounds__(kPrepThreads) void batch_prep_kernel(BaArgs a, int 
   __shared__ int32_t base_s[kBaMaxSegs + 2];
   __shared__ int64_t start_s[kPrepStarts];
   __shared__ int64_t part[kPrepWaves];
+  __shared__ __attribute__((aligned(16))) float rk_s[64 * 68];
   if ((int)blockIdx.x < n_lines) {
     if (blockIdx.x == 0) ba_lay_out<0>(a, base_s, start_s, part);
     else ba_lay_out<1>(a, base_s, start_s, part);
@@ -364,7 +382,7 @@ __global__ __launch_bounds__(kPrepThreads) void batch_prep_kernel(BaArgs a, int 
     return;
   }
   for (int64_t t = blk * kPrepThreads + threadIdx.x; t < a.n_tokens; t += n_blks * kPrepThreads) ba_find_token(a, (int)t);
-  ba_rotate_rows<DT>(a, blk, n_blks);
+  ba_rotate_rows<DT>(a, blk, n_blks, rk_s);
 }
 
 // ------------------------------------------------------------------------------- joining
@@ -411,13 +429,13 @@ __global__ __launch_bounds__(64 * kJoinWaves) void batch_join_kernel(BaArgs a) {
   const int64_t rowid = min(r0 + c, n_rows - 1);
   const int tok = (int)ba_div(rowid, a.hq), qh = (int)(rowid - (int64_t)tok * a.hq);
   const int h = qh / a.G, gq = qh - h * a.G;
-  // R_v's entries of this wave's dims, wanted last
-  float rv[16];
+  // R_v's operands of this wave's dims, wanted last
+  ba_v8h rv[2][2];
 #pragma unroll
-  for (int nb = 0; nb < 4; ++nb)
+  for (int part = 0; part < 2; ++part)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) rv[4 * nb + r] = a.vrot[(16 * nb + 4 * g + r) * a.vrot_row + (16 * wave + c) * a.vrot_col];
-
+    for (int s = 0; s < 2; ++s)
+      rv[part][s] = reinterpret_cast<const ba_v8h*>(a.vrot16)[(part * 8 + wave * 2 + s) * 64 + lane];
   const BaToken t = a.tokens[tok];
   BaFrom s{}, p{};
   if (t.seq < a.B) {
@@ -475,18 +493,43 @@ __global__ __launch_bounds__(64 * kJoinWaves) void batch_join_kernel(BaArgs a) {
     f[w] = __builtin_amdgcn_exp2f(stat_s[w][c][0] - Ms);
     L += stat_s[w][c][1] * f[w];
   }
-  // out_c[16 ob + 4 g + r] of lane (c, g) = sum over k-steps (nb, r) of A[c][g] =
-  // R_v[16 nb + 4 g + r][16 ob + c] and B[g][c] = O_c[16 nb + 4 g + r]
+  // ba_rotate_back for one ob, into fp16's range by a power of two of the row
   const float inv = L == 0.f ? 0.f : 1.f / L;
-  ba_v4f acc = {0.f, 0.f, 0.f, 0.f};
+  float x[16], xm = 0.f;
 #pragma unroll
   for (int nb = 0; nb < 4; ++nb) {
-    ba_v4f x = {0.f, 0.f, 0.f, 0.f};
+    ba_v4f v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < kJoinWaves; ++w) x += *reinterpret_cast<const ba_v4f*>(&sums_s[w][c][16 * nb + 4 * g]) * f[w];
+    for (int w = 0; w < kJoinWaves; ++w) v += *reinterpret_cast<const ba_v4f*>(&sums_s[w][c][16 * nb + 4 * g]) * f[w];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(rv[4 * nb + r], x[r] * inv, acc, 0, 0, 0);
+    for (int r = 0; r < 4; ++r) {
+      x[4 * nb + r] = v[r] * inv;
+      xm = fmaxf(xm, fabsf(x[4 * nb + r]));
+    }
   }
+  xm = fmaxf(xm, __shfl_xor(xm, 16, 64));
+  xm = fmaxf(xm, __shfl_xor(xm, 32, 64));
+  const int e = ba_exponent(xm);
+  const float up = ldexpf(1.f, 4 - e);
+  ba_v8h hi[2], lo[2];
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      _Float16 hv, lv;
+      split_f16(x[8 * s + i] * up, hv, lv);
+      hi[s][i] = hv;
+      lo[s][i] = lv;
+    }
+  mfma_operand_fence(hi[0], hi[1], lo[0], lo[1]);
+  ba_v4f acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(rv[1][s], hi[s], acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(rv[0][s], lo[s], acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(rv[0][s], hi[s], acc, 0, 0, 0);
+  }
+  acc *= ldexpf(1.f, e - 4);
   if (r0 + c >= n_rows) return;
   if (t.seq < a.B || a.zero_tail) ba_store(a, tok, qh, 16 * wave + 4 * g, acc);
   if (a.lse && wave == 0 && g == 0) a.lse[rowid] = ba_lse(M, L);
@@ -567,10 +610,10 @@ __global__ __launch_bounds__(64) void batch_join_cut_kernel(BaArgs a) {
 
 // Which kernels a call runs, and its workspace.
 struct BaPlan {
-  bool prec;
+  bool prec, pair;
   int rw[2], groups[2];  // per line: rows of a group of columns, groups
   int64_t items[2];
-  unsigned grid[2];
+  unsigned grid;
   int64_t segs[2];
 };
 
@@ -579,6 +622,7 @@ BaPlan ba_plan(tq_dtype q_dtype, int64_t n, int hq, int hkv, int64_t B, int64_t 
   p.prec = q_dtype != TQ_BF16;
   const int G = hq / hkv;
   const int64_t rows = n * G, cus = device_cu_count();
+  p.pair = n_groups > 0;
   p.segs[0] = B;
   p.segs[1] = n_groups;
   for (int l = 0; l < (n_groups > 0 ? 2 : 1); ++l) {
@@ -587,13 +631,13 @@ BaPlan ba_plan(tq_dtype q_dtype, int64_t n, int hq, int hkv, int64_t B, int64_t 
     // (rounded: a few rows of padding behind single tokens do not widen them)
     const int64_t segs = std::max<int64_t>(l ? n_groups : B, 1);
     const int64_t avg = std::max<int64_t>(1, (n + segs / 2) / segs) * G;
-    p.rw[l] = avg <= 4 ? 4 : avg <= 8 ? 8 : 16;
-    p.groups[l] = avg <= 16 ? 1 : kBaGroups;
+    p.rw[l] = l == 1 || avg > 8 ? 16 : avg <= 4 ? 4 : 8;
+    p.groups[l] = l == 1 || avg > 16 ? kBaGroups : 1;  // (groups hold many rows)
     const int R = p.rw[l] * p.groups[l];
     p.items[l] = rows / R + p.segs[l];
     // one workgroup per CU, fewer where even one-tile pieces would not fill them
     const int64_t pieces = p.items[l] * hkv * (capacity / 64 + 1 + kBaOver);
-    p.grid[l] = (unsigned)std::max<int64_t>(1, std::min(cus, pieces));
+    p.grid = std::max(p.grid, (unsigned)std::max<int64_t>(1, std::min(cus, pieces)));
   }
   return p;
 }
@@ -615,9 +659,9 @@ size_t ba_place(const BaPlan& p, int64_t n, int hq, char* at, BaArgs* a) {
   b.vrot16 = reinterpret_cast<_Float16*>(take(2 * 4096 * sizeof(_Float16)));
   if (p.prec) b.qlo = reinterpret_cast<_Float16*>(take(rows * 128));
   for (int l = 0; l < 2; ++l) {
-    if (p.grid[l] == 0) continue;
+    if (l == 1 && !p.pair) continue;
     BaLine& ln = b.line[l];
-    ln.waves = (int)p.grid[l] * ba_waves(p.prec, p.rw[l], p.groups[l]);
+    ln.waves = (int)p.grid * ba_waves(p.prec, p.rw[0], p.groups[0], p.pair);
     ln.rows = p.rw[l] * p.groups[l];
     ln.max_items = (int)p.items[l];
     ln.head = reinterpret_cast<BaHead*>(take(sizeof(BaHead)));
@@ -636,16 +680,16 @@ size_t ba_place(const BaPlan& p, int64_t n, int hq, char* at, BaArgs* a) {
 }
 
 template <int VB>
-void ba_run_bits(const BaArgs& a, int l, const BaPlan& p, hipStream_t st) {
+void ba_run_bits(const BaArgs& a, const BaPlan& p, hipStream_t st) {
   const bool wide = (uint64_t)a.num_blocks * a.hkv << a.bs_log2 > 0xFFFFFFFFu / 32;  // key bytes past 32 bits
-  if (a.bs_log2 < 6) ba_launch<VB, true>(a, l, wide, p.prec, p.rw[l], p.groups[l], p.grid[l], st);
-  else ba_launch<VB, false>(a, l, wide, p.prec, p.rw[l], p.groups[l], p.grid[l], st);
+  if (a.bs_log2 < 6) ba_launch<VB, true>(a, p.pair, wide, p.prec, p.rw[0], p.groups[0], p.grid, st);
+  else ba_launch<VB, false>(a, p.pair, wide, p.prec, p.rw[0], p.groups[0], p.grid, st);
 }
 
-void ba_run(int vbits, const BaArgs& a, int l, const BaPlan& p, hipStream_t st) {
-  if (vbits == 2) ba_run_bits<2>(a, l, p, st);
-  else if (vbits == 3) ba_run_bits<3>(a, l, p, st);
-  else ba_run_bits<4>(a, l, p, st);
+void ba_run(int vbits, const BaArgs& a, const BaPlan& p, hipStream_t st) {
+  if (vbits == 2) ba_run_bits<2>(a, p, st);
+  else if (vbits == 3) ba_run_bits<3>(a, p, st);
+  else ba_run_bits<4>(a, p, st);
 }
 
 }  // namespace
@@ -748,10 +792,8 @@ int tq_attention_batch_paged_dl(const void* q, tq_dtype q_dtype, int32_t n_token
   else if (q_dtype == TQ_F16) hipLaunchKernelGGL((batch_prep_kernel<TQ_F16>), prep, pthreads, 0, st, a, lines, vbits);
   else hipLaunchKernelGGL((batch_prep_kernel<TQ_BF16>), prep, pthreads, 0, st, a, lines, vbits);
   TQ_LAUNCH_CHECK("batch_prep_kernel");
-  for (int l = lines - 1; l >= 0; --l) {
-    ba_run(vbits, a, l, p, st);
-    TQ_LAUNCH_CHECK("batch_attn_kernel");
-  }
+  ba_run(vbits, a, p, st);
+  TQ_LAUNCH_CHECK("batch_attn_kernel");
   if (a.direct) {
     const dim3 cut((unsigned)((a.line[0].waves - 1) * p.groups[0] + kTailBlocks));
     if (p.prec) hipLaunchKernelGGL((batch_join_cut_kernel<true>), cut, dim3(64), 0, st, a);

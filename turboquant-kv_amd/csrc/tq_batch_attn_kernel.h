@@ -86,54 +86,48 @@ __device__ __forceinline__ float ba_max4(float x) {
   return ba_max(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
-// RW rows of 16 columns (16 / RW copies share a tile's tokens), NGR groups of columns.  WIDE: pools
-// of 4 GB and more, whose rows need 64-bit addresses.
-template <int VB, bool SUB, bool PREC, int RW, int NGR, bool WIDE>
-__global__ __launch_bounds__(64 * ba_waves(PREC, RW, NGR), ba_waves(PREC, RW, NGR) / 4) void batch_attn_kernel(BaArgs a, BaLine ln) {
+// Builds the tables in LDS from the entries that the preparing kernel made; every wave calls it
+// once, after asking for its first item's data.
+template <int VB, bool PREC, int WAVES>
+__device__ __forceinline__ void ba_build_tables(const BaArgs& a, uint8_t* smem) {
+  const int tid = threadIdx.x;
+  const int e = tid & 255;  // threads t, t + 256, .. write entry t's copies in turn, 16 bytes each
+  const BaEntry x = a.entries[e];
+#pragma unroll
+  for (int k = tid >> 8; k < 16; k += WAVES / 4) {
+    // rotated by the entry so that a wave's stores spread over the banks; PREC: the lo parts'
+    // copies fill the second 128 bytes
+    const int q = (k + e) & 15;
+    const bool second = PREC && q >= 8;
+    const uint32_t kx = second ? x.klo : x.khi;
+    const uint32_t v0 = second ? x.vlo[0] : x.vhi[0], v1 = VB == 2 ? (second ? x.vlo[1] : x.vhi[1]) : v0;
+    *reinterpret_cast<ba_u32x4*>(smem + e * 256 + 16 * q) = (ba_u32x4){kx, kx, kx, kx};
+    *reinterpret_cast<ba_u32x4*>(smem + kBaVTab + e * 256 + 16 * q) = (ba_u32x4){v0, v1, v0, v1};
+  }
+  __syncthreads();
+}
+
+// A wave's piece of line `ln`.  RW rows of 16 columns (16 / RW copies share a tile's tokens), NGR
+// groups of columns; WIDE: pools of 4 GB and more, whose rows need 64-bit addresses.
+template <int VB, bool SUB, bool PREC, int RW, int NGR, bool WIDE, int WAVES>
+__device__ __forceinline__ void ba_piece(const BaArgs& a, const BaLine& ln, uint8_t* smem, int w, bool& built) {
 #pragma clang fp contract(off)
   static_assert(NGR == 1 || RW == 16, "groups of columns hold 16 rows each");
   constexpr int NB = RW / 4;       // 16-token groups whose scores a lane keeps
   constexpr int R = RW * NGR;
-  constexpr int WAVES = ba_waves(PREC, RW, NGR);
-  __shared__ __attribute__((aligned(16))) uint8_t smem[kBaNorms + WAVES * 512];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, g = lane >> 4;
   const int cb = c / RW, cr = c % RW;  // the column's copy and row
   const int hkv = a.hkv, G = a.G;
-
-  // Neighbouring pieces on one XCD (workgroup w runs on XCD w % 8): rows of one prefix read the
-  // same tiles there, and adjacent KV heads of a 16-token block share lines of norms.  Few
-  // pieces spread over the workgroups.
-  const unsigned grid = gridDim.x;
-  const unsigned blk = grid % 8 == 0 ? (blockIdx.x % 8) * (grid / 8) + blockIdx.x / 8 : blockIdx.x;
-  if (ln.work[blk] < 0) return;  // the workgroup's first piece: it lies behind the line's end
-  const int w = wave * (int)grid + (int)blk;
   int item = __builtin_amdgcn_readfirstlane(ln.work[w]);
-  BaItem it = ln.items[max(item, 0)];
+  if (item < 0) return;
   auto uniform64 = [](int64_t x) {
     return (int64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)x) |
            (int64_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32;
   };
+  BaItem it = ln.items[item];
   const int64_t chunk = uniform64(ln.head->chunk), total = uniform64(ln.head->total);
-
-  // ---- the tables, from the entries that the preparing kernel made
-  {
-    const int e = tid & 255;  // threads t, t + 256, .. write entry t's copies in turn, 16 bytes each
-    const BaEntry x = a.entries[e];
-#pragma unroll
-    for (int k = tid >> 8; k < 16; k += WAVES / 4) {
-      // rotated by the entry so that a wave's stores spread over the banks; PREC: the lo parts'
-      // copies fill the second 128 bytes
-      const int q = (k + e) & 15;
-      const bool second = PREC && q >= 8;
-      const uint32_t kx = second ? x.klo : x.khi;
-      const uint32_t v0 = second ? x.vlo[0] : x.vhi[0], v1 = VB == 2 ? (second ? x.vlo[1] : x.vhi[1]) : v0;
-      *reinterpret_cast<ba_u32x4*>(smem + e * 256 + 16 * q) = (ba_u32x4){kx, kx, kx, kx};
-      *reinterpret_cast<ba_u32x4*>(smem + kBaVTab + e * 256 + 16 * q) = (ba_u32x4){v0, v1, v0, v1};
-    }
-    __syncthreads();
-  }
   const float vsc_inv = a.entries[0].vsc_inv;  // a power of two
   // this lane's copy of an entry's hi part (PREC: its lo part is 128 bytes on)
   const uint32_t koff = PREC ? 4u * (lane & 31) : 4u * lane;
@@ -150,7 +144,6 @@ __global__ __launch_bounds__(64 * ba_waves(PREC, RW, NGR), ba_waves(PREC, RW, NG
   };
 
 
-  if (item < 0) return;
   const int bsl = a.bs_log2;
   float* const snorm = reinterpret_cast<float*>(smem + kBaNorms) + wave * 128;
   const __amdgpu_buffer_rsrc_t krs = buf_rsrc(a.kpairs, 0xFFFFFFFFu), vrs = buf_rsrc(a.vtiles, 0xFFFFFFFFu);
@@ -578,9 +571,13 @@ __global__ __launch_bounds__(64 * ba_waves(PREC, RW, NGR), ba_waves(PREC, RW, NG
     };
 
     // two buffers, one tile ahead: the other waves of the SIMD cover the rest
+    Tile r0, r1;
+    if (nw > 0) load(0, r0);
+    if (!built) {  // while the first tile is on its way
+      ba_build_tables<VB, PREC, WAVES>(a, smem);
+      built = true;
+    }
     if (nw > 0) {
-      Tile r0, r1;
-      load(0, r0);
       int i = 0;
       for (; i + 1 < nw; i += 2) {
         load(i + 1, r1);
@@ -655,25 +652,50 @@ __global__ __launch_bounds__(64 * ba_waves(PREC, RW, NGR), ba_waves(PREC, RW, NG
   }
 }
 
-template <int VB, bool SUB, bool PREC, bool WIDE>
-void ba_launch_kind(const BaArgs& a, int l, int rw, int groups, unsigned grid, hipStream_t st) {
-  constexpr int N = kBaGroups;
-  const dim3 gr(grid), bl(64 * ba_waves(PREC, rw, groups));
-  const BaLine& ln = a.line[l];
-  if (groups > 1) hipLaunchKernelGGL((batch_attn_kernel<VB, SUB, PREC, 16, N, WIDE>), gr, bl, 0, st, a, ln);
-  else if (rw == 16) hipLaunchKernelGGL((batch_attn_kernel<VB, SUB, PREC, 16, 1, WIDE>), gr, bl, 0, st, a, ln);
-  else if (rw == 8) hipLaunchKernelGGL((batch_attn_kernel<VB, SUB, PREC, 8, 1, WIDE>), gr, bl, 0, st, a, ln);
-  else hipLaunchKernelGGL((batch_attn_kernel<VB, SUB, PREC, 4, 1, WIDE>), gr, bl, 0, st, a, ln);
+// Line 0 alone (PAIR: line 1, whose items hold many rows, before it: a wave goes on with its
+// piece of the sequences' line while others still read prefixes).
+template <int VB, bool SUB, bool PREC, int RW, int NGR, bool WIDE, bool PAIR>
+__global__ __launch_bounds__(64 * ba_waves(PREC, RW, NGR, PAIR), ba_waves(PREC, RW, NGR, PAIR) / 4)
+void batch_attn_kernel(BaArgs a) {
+  constexpr int WAVES = ba_waves(PREC, RW, NGR, PAIR);
+  __shared__ __attribute__((aligned(16))) uint8_t smem[kBaNorms + WAVES * 512];
+  // Neighbouring pieces on one XCD (workgroup w runs on XCD w % 8): rows of one prefix read the
+  // same tiles there, and adjacent KV heads of a 16-token block share lines of norms.  Few
+  // pieces spread over the workgroups.
+  const unsigned grid = gridDim.x;
+  const unsigned blk = grid % 8 == 0 ? (blockIdx.x % 8) * (grid / 8) + blockIdx.x / 8 : blockIdx.x;
+  // (a workgroup's first piece: where it lies behind the line's end, all do)
+  if (a.line[0].work[blk] < 0 && !(PAIR && a.line[1].work[blk] >= 0)) return;
+  const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)) * (int)grid + (int)blk;
+  bool built = false;
+  if constexpr (PAIR) ba_piece<VB, SUB, PREC, 16, kBaGroups, WIDE, WAVES>(a, a.line[1], smem, w, built);
+  ba_piece<VB, SUB, PREC, RW, NGR, WIDE, WAVES>(a, a.line[0], smem, w, built);
+  if (!built) ba_build_tables<VB, PREC, WAVES>(a, smem);
+}
+
+template <int VB, bool SUB, bool PREC, bool WIDE, bool PAIR>
+void ba_launch_kind(const BaArgs& a, int rw, int groups, unsigned grid, hipStream_t st) {
+  const dim3 gr(grid), bl(64 * ba_waves(PREC, rw, groups, PAIR));
+  if (groups > 1) hipLaunchKernelGGL((batch_attn_kernel<VB, SUB, PREC, 16, kBaGroups, WIDE, PAIR>), gr, bl, 0, st, a);
+  else if (rw == 16) hipLaunchKernelGGL((batch_attn_kernel<VB, SUB, PREC, 16, 1, WIDE, PAIR>), gr, bl, 0, st, a);
+  else if (rw == 8) hipLaunchKernelGGL((batch_attn_kernel<VB, SUB, PREC, 8, 1, WIDE, PAIR>), gr, bl, 0, st, a);
+  else hipLaunchKernelGGL((batch_attn_kernel<VB, SUB, PREC, 4, 1, WIDE, PAIR>), gr, bl, 0, st, a);
+}
+
+template <int VB, bool SUB, bool PAIR>
+void ba_launch_lines(const BaArgs& a, bool wide, bool prec, int rw, int groups, unsigned grid, hipStream_t st) {
+  if (wide && prec) ba_launch_kind<VB, SUB, true, true, PAIR>(a, rw, groups, grid, st);
+  else if (wide) ba_launch_kind<VB, SUB, false, true, PAIR>(a, rw, groups, grid, st);
+  else if (prec) ba_launch_kind<VB, SUB, true, false, PAIR>(a, rw, groups, grid, st);
+  else ba_launch_kind<VB, SUB, false, false, PAIR>(a, rw, groups, grid, st);
 }
 
 }  // namespace
 
 template <int VB, bool SUB>
-void ba_launch(const BaArgs& a, int l, bool wide, bool prec, int rw, int groups, unsigned grid, hipStream_t st) {
-  if (wide && prec) ba_launch_kind<VB, SUB, true, true>(a, l, rw, groups, grid, st);
-  else if (wide) ba_launch_kind<VB, SUB, false, true>(a, l, rw, groups, grid, st);
-  else if (prec) ba_launch_kind<VB, SUB, true, false>(a, l, rw, groups, grid, st);
-  else ba_launch_kind<VB, SUB, false, false>(a, l, rw, groups, grid, st);
+void ba_launch(const BaArgs& a, bool pair, bool wide, bool prec, int rw, int groups, unsigned grid, hipStream_t st) {
+  if (pair) ba_launch_lines<VB, SUB, true>(a, wide, prec, rw, groups, grid, st);
+  else ba_launch_lines<VB, SUB, false>(a, wide, prec, rw, groups, grid, st);
 }
 
 }  // namespace tq
