@@ -141,8 +141,8 @@ __device__ __forceinline__ void ba_lay_out(const BaArgs& a, int32_t* base_s, int
     }
     place += all;
   }
-  // Equal pieces, of a few tiles at least.
-  const int64_t chunk = max<int64_t>(kBaOver + 1, ba_div(place + ln.waves - 1, ln.waves));
+  // Equal pieces, of two tiles at least: a single one would double what is to be joined.
+  const int64_t chunk = max<int64_t>(2, ba_div(place + ln.waves - 1, ln.waves));
   if (tid == 0) *ln.head = BaHead{chunk, place, n_items, 0};
   // The item that each wave's piece begins in: a wave per item fills its waves' entries, or,
   // where items abound, each entry searches for its own.

@@ -10,6 +10,9 @@ namespace {
 constexpr int kBaVTab = 65536;
 constexpr int kBaNorms = 131072;  // [waves][2][64] floats
 
+// Weights reach 2^kBaSlack before their reference moves; norms are scaled down by as much less one.
+constexpr float kBaSlack = 4.f, kBaNormDown = 0.125f;
+
 __device__ __forceinline__ ba_v8h ba_h8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   ba_u32x4 t = {a, b, c, d};
   return __builtin_bit_cast(ba_v8h, t);
@@ -35,13 +38,19 @@ __device__ __forceinline__ float ba_softcap(float x, float cap2) {
   }
 }
 
-__device__ __forceinline__ int ba_wave_min(int v) {
+// The least (greatest) of v over RW neighbouring lanes, the rows of a group of columns; uniform.
+template <int RW>
+__device__ __forceinline__ int ba_rows_min(int v) {
 #pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
+  for (int o = RW / 2; o >= 1; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
   return __builtin_amdgcn_readfirstlane(v);
 }
-__device__ __forceinline__ int ba_wave_max(int v) { return -ba_wave_min(-v); }
-
+template <int RW>
+__device__ __forceinline__ int ba_rows_max(int v) {
+#pragma unroll
+  for (int o = RW / 2; o >= 1; o >>= 1) v = max(v, __shfl_xor(v, o, 64));
+  return __builtin_amdgcn_readfirstlane(v);
+}
 
 // Loads through a raw buffer resource: a lane's 32-bit offset plus a scalar one, no vector
 // address arithmetic.
@@ -50,13 +59,6 @@ __device__ __forceinline__ T ba_load(__amdgpu_buffer_rsrc_t rs, uint32_t lane_of
   if constexpr (sizeof(T) == 4) return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(rs, lane_off, off, 0));
   else if constexpr (sizeof(T) == 8) return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b64(rs, lane_off, off, 0));
   else return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b128(rs, lane_off, off, 0));
-}
-
-// fp16 products a u (low half) and b v, each rounded once.
-__device__ __forceinline__ uint32_t ba_products(float a, float u, float b, float v) {
-  uint32_t r;
-  asm("v_fma_mixlo_f16 %0, %1, %2, 0\n\tv_fma_mixhi_f16 %0, %3, %4, 0" : "=&v"(r) : "v"(a), "v"(u), "v"(b), "v"(v));
-  return r;
 }
 
 // fp16 hi and lo parts of a (low half) and b.  (Each is pinned as one fp32 value first: a product
@@ -171,6 +173,24 @@ __device__ __forceinline__ void ba_piece(const BaArgs& a, const BaLine& ln, uint
       continue;
     }
 
+    const int k0 = t0 + ta, nw = tb - ta;  // tiles of the piece
+    // Pool rows of 16 tiles' 16-token groups at a time (lane 4 i + b: tile i's group b), the next
+    // 16 tiles' block ids requested while these are used.
+    const int32_t* btab = a.block_tables + (int64_t)table * a.table_stride;
+    auto load_ids = [&](int chunk16) -> uint32_t {
+      const int i = min(chunk16 * 16 + (lane >> 2), nw - 1);
+      const int64_t tb = ((int64_t)(k0 + i) << 6) + 16 * (lane & 3);
+      const int bi = (int)min<int64_t>(tb >> bsl, (int64_t)a.max_blocks - 1);
+      return (uint32_t)btab[bi];
+    };
+    using row_t = std::conditional_t<WIDE, uint64_t, uint32_t>;
+    auto pool_row = [&](uint32_t id, int chunk16) -> row_t {
+      const uint32_t tb = ((uint32_t)(k0 + chunk16 * 16 + (lane >> 2)) << 6) + 16u * (lane & 3);
+      return (((row_t)min(id, a.num_blocks - 1u) * (uint32_t)hkv + (uint32_t)h) << bsl) + (tb & ((1u << bsl) - 1u));
+    };
+    uint32_t ids_next = 0;
+    if (nw > 0) ids_next = load_ids(0);
+
     auto place_of = [&](int j, int& tok, int& qh) {
       const int row = min(row0 + 16 * j + cr, lastrow), ti = row / G;
       tok = tok0 + ti;
@@ -202,7 +222,7 @@ __device__ __forceinline__ void ba_piece(const BaArgs& a, const BaLine& ln, uint
     // One power of two for all the wave's rows, so that it goes with the key norms: shorter queries
     // are scaled down to the longest's.  Errors stay under 2^-22 (bf16 queries: 2^-11) of a row's
     // own length down to lengths 2^-17 (2^-28) of the longest row's.
-    qtop = ba_wave_max(qtop);
+    qtop = ba_rows_max<RW>(qtop);
 #pragma unroll
     for (int j = 0; j < NGR; ++j)
       if (__any(qe[j] != qtop)) {
@@ -225,11 +245,10 @@ __device__ __forceinline__ void ba_piece(const BaArgs& a, const BaLine& ln, uint
       hi_min = min(hi_min, hi[j]);
       hi_max = max(hi_max, hi[j]);
     }
-    lo_min = ba_wave_min(lo_min);
-    lo_max = ba_wave_max(lo_max);
-    hi_min = ba_wave_min(hi_min);
-    hi_max = ba_wave_max(hi_max);
-    const int k0 = t0 + ta, nw = tb - ta;  // tiles of the piece
+    lo_min = ba_rows_min<RW>(lo_min);
+    lo_max = ba_rows_max<RW>(lo_max);
+    hi_min = ba_rows_min<RW>(hi_min);
+    hi_max = ba_rows_max<RW>(hi_max);
 
     float m[NGR], l[NGR];
     ba_v4f o[NGR][4];
@@ -242,20 +261,6 @@ __device__ __forceinline__ void ba_piece(const BaArgs& a, const BaLine& ln, uint
       for (int nb = 0; nb < 4; ++nb) o[j][nb] = (ba_v4f){0.f, 0.f, 0.f, 0.f};
     }
 
-    // Pool rows of 16 tiles' 16-token groups at a time (lane 4 i + b: tile i's group b), the next
-    // 16 tiles' block ids requested while these are used.
-    const int32_t* btab = a.block_tables + (int64_t)table * a.table_stride;
-    auto load_ids = [&](int chunk16) -> uint32_t {
-      const int i = min(chunk16 * 16 + (lane >> 2), nw - 1);
-      const int64_t tb = ((int64_t)(k0 + i) << 6) + 16 * (lane & 3);
-      const int bi = (int)min<int64_t>(tb >> bsl, (int64_t)a.max_blocks - 1);
-      return (uint32_t)btab[bi];
-    };
-    using row_t = std::conditional_t<WIDE, uint64_t, uint32_t>;
-    auto pool_row = [&](uint32_t id, int chunk16) -> row_t {
-      const uint32_t tb = ((uint32_t)(k0 + chunk16 * 16 + (lane >> 2)) << 6) + 16u * (lane & 3);
-      return (((row_t)min(id, a.num_blocks - 1u) * (uint32_t)hkv + (uint32_t)h) << bsl) + (tb & ((1u << bsl) - 1u));
-    };
     constexpr int NV = VB == 2 ? 4 : (SUB ? 8 : 2 * VB);
     struct Tile {
       ba_u32x2 kw[4];
@@ -263,8 +268,6 @@ __device__ __forceinline__ void ba_piece(const BaArgs& a, const BaLine& ln, uint
       uint32_t vw[NV];
     };
     row_t rows16 = 0;
-    uint32_t ids_next = 0;
-    if (nw > 0) ids_next = load_ids(0);
     // i: the wave's i-th tile, asked for in order (a repeated last one excepted)
     auto load = [&](int i, Tile& t) {
       if ((i & 15) == 0 && i < nw) {
@@ -350,7 +353,9 @@ __device__ __forceinline__ void ba_piece(const BaArgs& a, const BaLine& ln, uint
           for (int nb = 0; nb < 4; ++nb) o[j][nb] *= f;
       }
       snorm[lane] = t.nk * kscale;
-      snorm[64 + lane] = nvl * vs.s;
+      // (weights are at most 2^kBaSlack: their products with norms stay below 2^15)
+      if constexpr (PREC) snorm[64 + lane] = nvl * (vs.s * kBaNormDown);
+      else reinterpret_cast<_Float16*>(snorm + 64)[lane] = (_Float16)(nvl * (vs.s * kBaNormDown));
       __builtin_amdgcn_wave_barrier();
 
       // value word helpers: VB 3 / 4, tile word i of half s, and the word whose bytes index
@@ -459,9 +464,13 @@ __device__ __forceinline__ void ba_piece(const BaArgs& a, const BaLine& ln, uint
       }
 
       // ---- online softmax (log2 domain); weights times value norms as fp16
-      ba_v4f nv4[NB];
+      ba_v4f nv4[PREC ? NB : 1];
+      ba_u32x2 nvh[PREC ? 1 : NB];  // two fp16 a word
 #pragma unroll
-      for (int k = 0; k < NB; ++k) nv4[k] = *reinterpret_cast<const ba_v4f*>(snorm + 64 + tg + 16 * k);
+      for (int k = 0; k < NB; ++k) {
+        if constexpr (PREC) nv4[k] = *reinterpret_cast<const ba_v4f*>(snorm + 64 + tg + 16 * k);
+        else nvh[k] = *reinterpret_cast<const ba_u32x2*>(reinterpret_cast<const _Float16*>(snorm + 64) + tg + 16 * k);
+      }
       ba_v8h bh[NGR][2], bl[PREC ? NGR : 1][2];
 #pragma unroll
       for (int j = 0; j < NGR; ++j) {
@@ -470,16 +479,17 @@ __device__ __forceinline__ void ba_piece(const BaArgs& a, const BaLine& ln, uint
         for (int k = 0; k < NB; ++k)
 #pragma unroll
           for (int r = 0; r < 4; ++r) mx = fmaxf(mx, sv[j][k][r]);
-        mx = ba_max4(mx);
-        const float mn = fmaxf(m[j], mx);
-        const float ms = mn == -INFINITY ? 0.f : mn;
-        if (__any(mn != m[j])) {
-          const float alpha = __builtin_amdgcn_exp2f(m[j] - ms);
+        // The weights' reference m[j] follows the maximum only when a score passes it by kBaSlack:
+        // most tiles neither exchange maxima between lanes nor rescale.
+        if (__any(mx > m[j] + kBaSlack)) {
+          const float mn = ba_max4(ba_max(mx, m[j]));
+          const float alpha = __builtin_amdgcn_exp2f(m[j] - (mn == -INFINITY ? 0.f : mn));
           l[j] *= alpha;
 #pragma unroll
           for (int nb = 0; nb < 4; ++nb) o[j][nb] *= alpha;
+          m[j] = mn;
         }
-        m[j] = mn;
+        const float ms = m[j] == -INFINITY ? 0.f : m[j];
         // weights times value norms, two fp16 a word: word q of group k holds tokens 2 q, 2 q + 1
         uint32_t ph[NB][2], pl[PREC ? NB : 1][2];
 #pragma unroll
@@ -489,9 +499,17 @@ __device__ __forceinline__ void ba_piece(const BaArgs& a, const BaLine& ln, uint
             // results below 2^-126 flush to 0: nothing beside the running maximum's 1
             const float pa = __builtin_amdgcn_exp2f(sv[j][k][2 * q] - ms);
             const float pb = __builtin_amdgcn_exp2f(sv[j][k][2 * q + 1] - ms);
-            l[j] += pa + pb;
-            if constexpr (PREC) ba_split(pa * nv4[k][2 * q], pb * nv4[k][2 * q + 1], ph[k][q], pl[k][q]);
-            else ph[k][q] = ba_products(pa, nv4[k][2 * q], pb, nv4[k][2 * q + 1]);
+            if constexpr (PREC) {
+              l[j] += pa + pb;
+              ba_split(pa * nv4[k][2 * q], pb * nv4[k][2 * q + 1], ph[k][q], pl[k][q]);
+            } else {  // the sum of the weights as they are rounded
+              typedef float v2f __attribute__((ext_vector_type(2)));
+              typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+              const v2h p = __builtin_convertvector((v2f){pa, pb}, v2h);
+              l[j] = __builtin_amdgcn_fdot2(p, (v2h){(_Float16)1.f, (_Float16)1.f}, l[j], false);
+              const uint32_t nv2 = nvh[k][q];  // (a bit cast of the vector's element itself reads element 0)
+              ph[k][q] = __builtin_bit_cast(uint32_t, p * __builtin_bit_cast(v2h, nv2));
+            }
           }
         if (__builtin_expect(odd, 0)) {  // rows that do not see it must not take 0 * inf
           asm volatile("");
@@ -590,7 +608,7 @@ __device__ __forceinline__ void ba_piece(const BaArgs& a, const BaLine& ln, uint
 
     if (next) it = ln.items[++item];
     // ---- the piece's sums: over the row's lanes and, for few rows, its copies
-    const float vinv = vs.inv() * vsc_inv;
+    const float vinv = vs.inv() * vsc_inv * (1.f / kBaNormDown);
 #pragma unroll
     for (int j = 0; j < NGR; ++j) {
       l[j] += __shfl_xor(l[j], 16, 64);
@@ -598,7 +616,7 @@ __device__ __forceinline__ void ba_piece(const BaArgs& a, const BaLine& ln, uint
       float f = vinv;
       const bool done = NGR > 1 && whole && a.direct;
       if constexpr (NGR > 1) {
-        if (done) {  // (sums over the weights' total: at most 2^14 in the norms' scale)
+        if (done) {  // (sums over the weights' total: at most 2^11 in the norms' scale)
           const float inv = l[j] == 0.f ? 0.f : 1.f / l[j];
           ba_v4f x[4], out[4];
 #pragma unroll
