@@ -56,7 +56,10 @@ constexpr int ba_waves(bool prec, int rw, int groups, bool pair) {
 constexpr int kBaMaxSegs = 8191;  // sequences or groups of a call: the preparing kernel's LDS
 constexpr int kBaQueryTop = 14;   // rotated queries are scaled to at most 2^14 (fp16's range ends at 2^16)
 constexpr int kBaOver = 3;        // an (item, head)'s cost besides its tiles, in tiles
-constexpr int kBaGroups = 2;      // groups of 16 rows a wave takes where rows abound: three spill
+// Groups of 16 rows that a wave takes where rows abound.  Three share a tile's lookups best where
+// their registers allow (bf16 queries without prefix groups: prompts 446 -> 395 us for three
+// spilling 40 values outside the loop; beside a second line 60 -> 63 us).
+constexpr int ba_groups(bool prec, bool pair) { return prec || pair ? 2 : 3; }
 // Floats of a partial slot of R rows: sums [R][64], (maximum, sum) [R][2].
 constexpr int ba_slot_floats(int R) { return R * 66; }
 

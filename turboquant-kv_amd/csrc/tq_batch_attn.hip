@@ -632,7 +632,7 @@ BaPlan ba_plan(tq_dtype q_dtype, int64_t n, int hq, int hkv, int64_t B, int64_t 
     const int64_t segs = std::max<int64_t>(l ? n_groups : B, 1);
     const int64_t avg = std::max<int64_t>(1, (n + segs / 2) / segs) * G;
     p.rw[l] = l == 1 || avg > 8 ? 16 : avg <= 4 ? 4 : 8;
-    p.groups[l] = l == 1 || avg > 16 ? kBaGroups : 1;  // (groups hold many rows)
+    p.groups[l] = l == 1 || avg > 16 ? ba_groups(p.prec, p.pair) : 1;  // (groups hold many rows)
     const int R = p.rw[l] * p.groups[l];
     p.items[l] = rows / R + p.segs[l];
     // one workgroup per CU, fewer where even one-tile pieces would not fill them

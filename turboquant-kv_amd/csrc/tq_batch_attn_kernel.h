@@ -6,9 +6,14 @@
 namespace tq {
 namespace {
 
-// LDS: key table, value table, each wave's norms of a tile.
+// LDS: key table, value table, each wave's norms of a tile.  An entry has 256 bytes of copies, or
+// (PREC) 128 of its hi part, and its lo part's kBaLo bytes from them: in the second half of the
+// eighth entry on (the last keys' in the first value entries').  Nearer, the compiler would read
+// both parts with one instruction, side by side, and move them to the operands they belong to:
+// 96 moves a tile.
 constexpr int kBaVTab = 65536;
-constexpr int kBaNorms = 131072;  // [waves][2][64] floats
+constexpr int kBaLo = 2048 + 128;
+constexpr int kBaNorms = 131072 + 2048;  // [waves][2][64] floats
 
 // Weights reach 2^kBaSlack before their reference moves; norms are scaled down by as much less one.
 constexpr float kBaSlack = 4.f, kBaNormDown = 0.125f;
@@ -97,14 +102,14 @@ __device__ __forceinline__ void ba_build_tables(const BaArgs& a, uint8_t* smem) 
   const BaEntry x = a.entries[e];
 #pragma unroll
   for (int k = tid >> 8; k < 16; k += WAVES / 4) {
-    // rotated by the entry so that a wave's stores spread over the banks; PREC: the lo parts'
-    // copies fill the second 128 bytes
+    // rotated by the entry so that a wave's stores spread over the banks
     const int q = (k + e) & 15;
     const bool second = PREC && q >= 8;
     const uint32_t kx = second ? x.klo : x.khi;
     const uint32_t v0 = second ? x.vlo[0] : x.vhi[0], v1 = VB == 2 ? (second ? x.vlo[1] : x.vhi[1]) : v0;
-    *reinterpret_cast<ba_u32x4*>(smem + e * 256 + 16 * q) = (ba_u32x4){kx, kx, kx, kx};
-    *reinterpret_cast<ba_u32x4*>(smem + kBaVTab + e * 256 + 16 * q) = (ba_u32x4){v0, v1, v0, v1};
+    const int at = e * 256 + 16 * q + (second ? kBaLo - 128 : 0);
+    *reinterpret_cast<ba_u32x4*>(smem + at) = (ba_u32x4){kx, kx, kx, kx};
+    *reinterpret_cast<ba_u32x4*>(smem + kBaVTab + at) = (ba_u32x4){v0, v1, v0, v1};
   }
   __syncthreads();
 }
@@ -131,7 +136,7 @@ __device__ __forceinline__ void ba_piece(const BaArgs& a, const BaLine& ln, uint
   BaItem it = ln.items[item];
   const int64_t chunk = uniform64(ln.head->chunk), total = uniform64(ln.head->total);
   const float vsc_inv = a.entries[0].vsc_inv;  // a power of two
-  // this lane's copy of an entry's hi part (PREC: its lo part is 128 bytes on)
+  // this lane's copy of an entry's hi part
   const uint32_t koff = PREC ? 4u * (lane & 31) : 4u * lane;
   // (byte 1: the value table's 64 KB, byte 2 of its addresses)
   const uint32_t voff = (VB == 2 ? (PREC ? 8u * (lane & 15) : 8u * (lane & 31)) : koff) | 0x100u;
@@ -401,8 +406,8 @@ __device__ __forceinline__ void ba_piece(const BaArgs& a, const BaLine& ln, uint
 #pragma unroll
           for (int j = 0; j < NGR; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, qhi[j][s], acc[j], 0, 0, 0);
           if constexpr (PREC) {
-            const ba_v8h al = ba_h8(*reinterpret_cast<const uint32_t*>(p0a + 128), *reinterpret_cast<const uint32_t*>(p1a + 128),
-                                    *reinterpret_cast<const uint32_t*>(p2a + 128), *reinterpret_cast<const uint32_t*>(p3a + 128));
+            const ba_v8h al = ba_h8(*reinterpret_cast<const uint32_t*>(p0a + kBaLo), *reinterpret_cast<const uint32_t*>(p1a + kBaLo),
+                                    *reinterpret_cast<const uint32_t*>(p2a + kBaLo), *reinterpret_cast<const uint32_t*>(p3a + kBaLo));
 #pragma unroll
             for (int j = 0; j < NGR; ++j) {
               acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, qlo[j][s], acc[j], 0, 0, 0);
@@ -539,7 +544,9 @@ __device__ __forceinline__ void ba_piece(const BaArgs& a, const BaLine& ln, uint
         }
       }
       // wait states between the conversions and the products that read them
-      if constexpr (NGR == 2 && PREC) {
+      if constexpr (NGR == 3) {
+        mfma_operand_fence6(bh[0][0], bh[0][1], bh[1][0], bh[1][1], bh[2][0], bh[2][1]);
+      } else if constexpr (NGR == 2 && PREC) {
         mfma_operand_fence8(bh[0][0], bh[0][1], bh[1][0], bh[1][1], bl[0][0], bl[0][1], bl[1][0], bl[1][1]);
       } else {
 #pragma unroll
@@ -561,7 +568,7 @@ __device__ __forceinline__ void ba_piece(const BaArgs& a, const BaLine& ln, uint
             const ba_u32x2 e0 = *reinterpret_cast<const ba_u32x2*>(q0), e1 = *reinterpret_cast<const ba_u32x2*>(q1);
             ah = ba_h8(e0.x, e0.y, e1.x, e1.y);
             if constexpr (PREC) {
-              const ba_u32x2 f0 = *reinterpret_cast<const ba_u32x2*>(q0 + 128), f1 = *reinterpret_cast<const ba_u32x2*>(q1 + 128);
+              const ba_u32x2 f0 = *reinterpret_cast<const ba_u32x2*>(q0 + kBaLo), f1 = *reinterpret_cast<const ba_u32x2*>(q1 + kBaLo);
               al = ba_h8(f0.x, f0.y, f1.x, f1.y);
             }
           } else {
@@ -573,8 +580,8 @@ __device__ __forceinline__ void ba_piece(const BaArgs& a, const BaLine& ln, uint
             ah = ba_h8(*reinterpret_cast<const uint32_t*>(q0), *reinterpret_cast<const uint32_t*>(q1),
                        *reinterpret_cast<const uint32_t*>(q2), *reinterpret_cast<const uint32_t*>(q3));
             if constexpr (PREC)
-              al = ba_h8(*reinterpret_cast<const uint32_t*>(q0 + 128), *reinterpret_cast<const uint32_t*>(q1 + 128),
-                         *reinterpret_cast<const uint32_t*>(q2 + 128), *reinterpret_cast<const uint32_t*>(q3 + 128));
+              al = ba_h8(*reinterpret_cast<const uint32_t*>(q0 + kBaLo), *reinterpret_cast<const uint32_t*>(q1 + kBaLo),
+                         *reinterpret_cast<const uint32_t*>(q2 + kBaLo), *reinterpret_cast<const uint32_t*>(q3 + kBaLo));
           }
 #pragma unroll
           for (int j = 0; j < NGR; ++j) {
@@ -686,7 +693,7 @@ void batch_attn_kernel(BaArgs a) {
   if (a.line[0].work[blk] < 0 && !(PAIR && a.line[1].work[blk] >= 0)) return;
   const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)) * (int)grid + (int)blk;
   bool built = false;
-  if constexpr (PAIR) ba_piece<VB, SUB, PREC, 16, kBaGroups, WIDE, WAVES>(a, a.line[1], smem, w, built);
+  if constexpr (PAIR) ba_piece<VB, SUB, PREC, 16, ba_groups(PREC, true), WIDE, WAVES>(a, a.line[1], smem, w, built);
   ba_piece<VB, SUB, PREC, RW, NGR, WIDE, WAVES>(a, a.line[0], smem, w, built);
   if (!built) ba_build_tables<VB, PREC, WAVES>(a, smem);
 }
@@ -694,7 +701,7 @@ void batch_attn_kernel(BaArgs a) {
 template <int VB, bool SUB, bool PREC, bool WIDE, bool PAIR>
 void ba_launch_kind(const BaArgs& a, int rw, int groups, unsigned grid, hipStream_t st) {
   const dim3 gr(grid), bl(64 * ba_waves(PREC, rw, groups, PAIR));
-  if (groups > 1) hipLaunchKernelGGL((batch_attn_kernel<VB, SUB, PREC, 16, kBaGroups, WIDE, PAIR>), gr, bl, 0, st, a);
+  if (groups > 1) hipLaunchKernelGGL((batch_attn_kernel<VB, SUB, PREC, 16, ba_groups(PREC, PAIR), WIDE, PAIR>), gr, bl, 0, st, a);
   else if (rw == 16) hipLaunchKernelGGL((batch_attn_kernel<VB, SUB, PREC, 16, 1, WIDE, PAIR>), gr, bl, 0, st, a);
   else if (rw == 8) hipLaunchKernelGGL((batch_attn_kernel<VB, SUB, PREC, 8, 1, WIDE, PAIR>), gr, bl, 0, st, a);
   else hipLaunchKernelGGL((batch_attn_kernel<VB, SUB, PREC, 4, 1, WIDE, PAIR>), gr, bl, 0, st, a);
