@@ -72,7 +72,7 @@ def build(verbose: bool = False) -> None:
     os.makedirs(OBJDIR, exist_ok=True)
     objs = []
     jobs = []
-    with cf.ThreadPoolExecutor(max_workers=4) as ex:
+    with cf.ThreadPoolExecutor(max_workers=8) as ex:
         for src in HIP_SOURCES:
             obj = os.path.join(OBJDIR, src.replace(".hip", ".o"))
             objs.append(obj)

@@ -47,12 +47,9 @@
 
 namespace tq {
 
-// Waves of a workgroup (one per CU: the tables fill its LDS).  Single tokens of fp32 / fp16
-// queries: 12 (168 registers a wave) instead of 8 hide more of the three products' latency: 48
-// sequences of up to 32k tokens, 4-bit values, 128 -> 117 us; bf16: 89 and 91 us.
-constexpr int ba_waves(bool prec, int rw, int groups, bool pair) {
-  return prec && groups == 1 && rw < 16 && !pair ? 12 : 8;
-}
+// Waves of a workgroup (one per CU: the tables fill its LDS).  256 registers a wave; 12 waves of 168
+// were no faster (48 sequences of up to 32k tokens: 89 and 91 us) and leave more to be joined.
+constexpr int kBaWaves = 8;
 constexpr int kBaMaxSegs = 8191;  // sequences or groups of a call: the preparing kernel's LDS
 constexpr int kBaQueryTop = 14;   // rotated queries are scaled to at most 2^14 (fp16's range ends at 2^16)
 constexpr int kBaOver = 3;        // an (item, head)'s cost besides its tiles, in tiles

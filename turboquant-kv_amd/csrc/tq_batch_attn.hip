@@ -661,7 +661,7 @@ size_t ba_place(const BaPlan& p, int64_t n, int hq, char* at, BaArgs* a) {
   for (int l = 0; l < 2; ++l) {
     if (l == 1 && !p.pair) continue;
     BaLine& ln = b.line[l];
-    ln.waves = (int)p.grid * ba_waves(p.prec, p.rw[0], p.groups[0], p.pair);
+    ln.waves = (int)p.grid * kBaWaves;
     ln.rows = p.rw[l] * p.groups[l];
     ln.max_items = (int)p.items[l];
     ln.head = reinterpret_cast<BaHead*>(take(sizeof(BaHead)));

@@ -23,24 +23,34 @@ __device__ __forceinline__ ba_v8h ba_h8(uint32_t a, uint32_t b, uint32_t c, uint
   return __builtin_bit_cast(ba_v8h, t);
 }
 
-// cap2 tanh(z) of x = 2 z log2(e).  tanh z = 1 - 2 / (1 + e^(2 z)), exact at both ends (the
-// exponential overflows to inf or vanishes); its absolute error of about 2^-23 is cap2 2^-23 in
-// the score.  EXACT: below |z| = 0.3 the odd series instead (the next term is 6e-10 relative),
-// whose error is relative.
-template <bool EXACT>
-__device__ __forceinline__ float ba_softcap(float x, float cap2) {
-  const float big = fmaf(-2.f * cap2, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x)), cap2);
-  if constexpr (!EXACT) {
-    return big;
+// cap2 tanh(z) of x = 2 z log2(e), in two forms.  Small: z times a polynomial in z^2 -- the odd
+// series up to z^11 (the next term is 6e-10 relative at |z| = 0.3), or, for bf16 queries, up to
+// z^5 with the z^7 term economized over |z| <= 0.3 (3e-6 relative): four instructions.  Any:
+// tanh z = 1 - 2 / (1 + e^(2 z)), exact at both ends (the exponential overflows to inf or
+// vanishes), whose absolute error of about 2^-23 is cap2 2^-23 in the score.
+constexpr float kBaSmallCap = 0.3f * 2.885390081777927f;
+template <bool PREC>
+__device__ __forceinline__ float ba_softcap_small(float x, float cap2) {
+  constexpr float h = 0.34657359027997264f;  // z / x
+  const float w = x * x;
+  if constexpr (PREC) {
+    constexpr float h2 = h * h, h4 = h2 * h2;
+    float p = fmaf(w, -0.00886323552990f * h4 * h4 * h2, 0.0218694885361f * h4 * h4);
+    p = fmaf(w, p, -0.0539682539683f * h4 * h2);
+    p = fmaf(w, p, 0.133333333333f * h4);
+    p = fmaf(w, p, -0.333333333333f * h2);
+    const float y = x * (h * cap2);
+    return fmaf(y * w, p, y);
   } else {
-    const float z = x * 0.34657359027997264f, w = z * z;
-    float p = fmaf(w, -0.00886323552990f, 0.0218694885361f);
-    p = fmaf(w, p, -0.0539682539683f);
-    p = fmaf(w, p, 0.133333333333f);
-    p = fmaf(w, p, -0.333333333333f);
-    const float y = z * cap2, small = fmaf(y * w, p, y);
-    return w < 0.09f ? small : big;
+    const float k = h * cap2;
+    const float p = fmaf(w, k * (0.126048f * h * h * h * h), k * (-0.333087f * h * h));
+    return x * fmaf(w, p, k * 0.9999988f);
   }
+}
+template <bool PREC>
+__device__ __forceinline__ float ba_softcap_any(float x, float cap2) {
+  const float big = fmaf(-2.f * cap2, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x)), cap2);
+  return PREC && fabsf(x) < kBaSmallCap ? ba_softcap_small<true>(x, cap2) : big;
 }
 
 // The least (greatest) of v over RW neighbouring lanes, the rows of a group of columns; uniform.
@@ -95,13 +105,13 @@ __device__ __forceinline__ float ba_max4(float x) {
 
 // Builds the tables in LDS from the entries that the preparing kernel made; every wave calls it
 // once, after asking for its first item's data.
-template <int VB, bool PREC, int WAVES>
+template <int VB, bool PREC>
 __device__ __forceinline__ void ba_build_tables(const BaArgs& a, uint8_t* smem) {
   const int tid = threadIdx.x;
   const int e = tid & 255;  // threads t, t + 256, .. write entry t's copies in turn, 16 bytes each
   const BaEntry x = a.entries[e];
 #pragma unroll
-  for (int k = tid >> 8; k < 16; k += WAVES / 4) {
+  for (int k = tid >> 8; k < 16; k += kBaWaves / 4) {
     // rotated by the entry so that a wave's stores spread over the banks
     const int q = (k + e) & 15;
     const bool second = PREC && q >= 8;
@@ -115,8 +125,9 @@ __device__ __forceinline__ void ba_build_tables(const BaArgs& a, uint8_t* smem) 
 }
 
 // A wave's piece of line `ln`.  RW rows of 16 columns (16 / RW copies share a tile's tokens), NGR
-// groups of columns; WIDE: pools of 4 GB and more, whose rows need 64-bit addresses.
-template <int VB, bool SUB, bool PREC, int RW, int NGR, bool WIDE, int WAVES>
+// groups of columns; WIDE: pools of 4 GB and more, whose rows need 64-bit addresses; MODS: scores
+// may be capped or biased.
+template <int VB, bool SUB, bool PREC, int RW, int NGR, bool WIDE, bool MODS>
 __device__ __forceinline__ void ba_piece(const BaArgs& a, const BaLine& ln, uint8_t* smem, int w, bool& built) {
 #pragma clang fp contract(off)
   static_assert(NGR == 1 || RW == 16, "groups of columns hold 16 rows each");
@@ -217,7 +228,7 @@ __device__ __forceinline__ void ba_piece(const BaArgs& a, const BaLine& ln, uint
       const int64_t rowid = (int64_t)tok * a.hq + qh;
       qe[j] = a.qexp[rowid];
       qtop = max(qtop, qe[j]);
-      slope[j] = a.slopes ? a.slopes[qh] * 1.4426950408889634f : 0.f;
+      slope[j] = MODS && a.slopes ? a.slopes[qh] * 1.4426950408889634f : 0.f;
 #pragma unroll
       for (int s = 0; s < 2; ++s) {  // dims 16 g + 8 s ..
         qhi[j][s] = *reinterpret_cast<const ba_v8h*>(a.qhi + rowid * 64 + 16 * g + 8 * s);
@@ -241,7 +252,7 @@ __device__ __forceinline__ void ba_piece(const BaArgs& a, const BaLine& ln, uint
           }
       }
     // the key norms' factor: scores in the log2 domain, or what ba_softcap takes
-    const float kscale = __builtin_amdgcn_ldexpf(a.cap2 != 0.f ? 2.885390081777927f * a.cap2_inv : 1.f, qtop);
+    const float kscale = __builtin_amdgcn_ldexpf(MODS && a.cap2 != 0.f ? 2.885390081777927f * a.cap2_inv : 1.f, qtop);
     int lo_min = INT_MAX, lo_max = 0, hi_min = INT_MAX, hi_max = 0;
 #pragma unroll
     for (int j = 0; j < NGR; ++j) {
@@ -390,33 +401,39 @@ __device__ __forceinline__ void ba_piece(const BaArgs& a, const BaLine& ln, uint
       // ---- scores: entry k of a lane is its copy's 16-token group NB cb + k
       ba_v4f sv[NGR][NB], all[NGR][4];
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        ba_v4f acc[NGR];
+      for (int j = 0; j < NGR; ++j)
 #pragma unroll
-        for (int j = 0; j < NGR; ++j) acc[j] = (ba_v4f){0.f, 0.f, 0.f, 0.f};
+        for (int b = 0; b < 4; ++b) all[j][b] = (ba_v4f){0.f, 0.f, 0.f, 0.f};
+      // (KB 16-token groups at a time, so that products of one sum do not follow each other)
+      constexpr int KB = NGR == 1 ? 4 : 1;
+#pragma unroll
+      for (int b0 = 0; b0 < 4; b0 += KB) {
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-          const uint32_t kw = t.kw[b][s];
-          const uint8_t* p0a = smem + kaddr(kw, 0);
-          const uint8_t* p1a = smem + kaddr(kw, 1);
-          const uint8_t* p2a = smem + kaddr(kw, 2);
-          const uint8_t* p3a = smem + kaddr(kw, 3);
-          const ba_v8h ah = ba_h8(*reinterpret_cast<const uint32_t*>(p0a), *reinterpret_cast<const uint32_t*>(p1a),
-                                  *reinterpret_cast<const uint32_t*>(p2a), *reinterpret_cast<const uint32_t*>(p3a));
+          ba_v8h ah[KB], al[PREC ? KB : 1];
 #pragma unroll
-          for (int j = 0; j < NGR; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, qhi[j][s], acc[j], 0, 0, 0);
-          if constexpr (PREC) {
-            const ba_v8h al = ba_h8(*reinterpret_cast<const uint32_t*>(p0a + kBaLo), *reinterpret_cast<const uint32_t*>(p1a + kBaLo),
-                                    *reinterpret_cast<const uint32_t*>(p2a + kBaLo), *reinterpret_cast<const uint32_t*>(p3a + kBaLo));
-#pragma unroll
-            for (int j = 0; j < NGR; ++j) {
-              acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, qlo[j][s], acc[j], 0, 0, 0);
-              acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(al, qhi[j][s], acc[j], 0, 0, 0);
-            }
+          for (int b = 0; b < KB; ++b) {
+            const uint32_t kw = t.kw[b0 + b][s];
+            const uint8_t* p0a = smem + kaddr(kw, 0);
+            const uint8_t* p1a = smem + kaddr(kw, 1);
+            const uint8_t* p2a = smem + kaddr(kw, 2);
+            const uint8_t* p3a = smem + kaddr(kw, 3);
+            ah[b] = ba_h8(*reinterpret_cast<const uint32_t*>(p0a), *reinterpret_cast<const uint32_t*>(p1a),
+                          *reinterpret_cast<const uint32_t*>(p2a), *reinterpret_cast<const uint32_t*>(p3a));
+            if constexpr (PREC)
+              al[b] = ba_h8(*reinterpret_cast<const uint32_t*>(p0a + kBaLo), *reinterpret_cast<const uint32_t*>(p1a + kBaLo),
+                            *reinterpret_cast<const uint32_t*>(p2a + kBaLo), *reinterpret_cast<const uint32_t*>(p3a + kBaLo));
           }
-        }
 #pragma unroll
-        for (int j = 0; j < NGR; ++j) all[j][b] = acc[j];
+          for (int p = 0; p < (PREC ? 3 : 1); ++p)
+#pragma unroll
+            for (int b = 0; b < KB; ++b)
+#pragma unroll
+              for (int j = 0; j < NGR; ++j)
+                all[j][b0 + b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p == 2 ? al[PREC ? b : 0] : ah[b],
+                                                                        p == 1 ? qlo[PREC ? j : 0][s] : qhi[j][s],
+                                                                        all[j][b0 + b], 0, 0, 0);
+        }
       }
 #pragma unroll
       for (int j = 0; j < NGR; ++j)
@@ -438,15 +455,30 @@ __device__ __forceinline__ void ba_piece(const BaArgs& a, const BaLine& ln, uint
 #pragma unroll
           for (int r = 0; r < 4; ++r) sv[j][k][r] *= nk4[r];
       }
-      if (a.cap2 != 0.f) {
+      if (MODS && a.cap2 != 0.f) {  // most tiles hold no score near the cap
 #pragma unroll
-        for (int j = 0; j < NGR; ++j)
+        for (int j = 0; j < NGR; ++j) {
+          float far = 0.f;
 #pragma unroll
           for (int k = 0; k < NB; ++k)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) sv[j][k][r] = ba_softcap<PREC>(sv[j][k][r], a.cap2);
+            for (int r = 0; r < 4; ++r) far = fmaxf(far, fabsf(sv[j][k][r]));
+          if (__any(far >= kBaSmallCap)) {
+            asm volatile("");
+#pragma unroll
+            for (int k = 0; k < NB; ++k)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) sv[j][k][r] = ba_softcap_any<PREC>(sv[j][k][r], a.cap2);
+          } else {
+            asm volatile("");
+#pragma unroll
+            for (int k = 0; k < NB; ++k)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) sv[j][k][r] = ba_softcap_small<PREC>(sv[j][k][r], a.cap2);
+          }
+        }
       }
-      if (a.slopes) {
+      if (MODS && a.slopes) {
 #pragma unroll
         for (int j = 0; j < NGR; ++j) {
           const float d0 = (float)(p0 + tg - qpos[j]);
@@ -556,61 +588,87 @@ __device__ __forceinline__ void ba_piece(const BaArgs& a, const BaLine& ln, uint
         }
       }
 
-      // ---- values
+      // ---- values (VN groups of 16 dims at a time, as above)
+      constexpr int VN = NGR == 1 ? 4 : 1;
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
 #pragma unroll
-        for (int nb = 0; nb < 4; ++nb) {
-          ba_v8h ah, al;
-          if constexpr (VB == 2) {
-            const uint8_t* q0 = smem + vaddr(t.vw[2 * s], nb);
-            const uint8_t* q1 = smem + vaddr(t.vw[2 * s + 1], nb);
-            const ba_u32x2 e0 = *reinterpret_cast<const ba_u32x2*>(q0), e1 = *reinterpret_cast<const ba_u32x2*>(q1);
-            ah = ba_h8(e0.x, e0.y, e1.x, e1.y);
-            if constexpr (PREC) {
-              const ba_u32x2 f0 = *reinterpret_cast<const ba_u32x2*>(q0 + kBaLo), f1 = *reinterpret_cast<const ba_u32x2*>(q1 + kBaLo);
-              al = ba_h8(f0.x, f0.y, f1.x, f1.y);
+        for (int n0 = 0; n0 < 4; n0 += VN) {
+          ba_v8h ah[VN], al[PREC ? VN : 1];
+#pragma unroll
+          for (int n = 0; n < VN; ++n) {
+            const int nb = n0 + n;
+            if constexpr (VB == 2) {
+              const uint8_t* q0 = smem + vaddr(t.vw[2 * s], nb);
+              const uint8_t* q1 = smem + vaddr(t.vw[2 * s + 1], nb);
+              const ba_u32x2 e0 = *reinterpret_cast<const ba_u32x2*>(q0), e1 = *reinterpret_cast<const ba_u32x2*>(q1);
+              ah[n] = ba_h8(e0.x, e0.y, e1.x, e1.y);
+              if constexpr (PREC) {
+                const ba_u32x2 f0 = *reinterpret_cast<const ba_u32x2*>(q0 + kBaLo);
+                const ba_u32x2 f1 = *reinterpret_cast<const ba_u32x2*>(q1 + kBaLo);
+                al[n] = ba_h8(f0.x, f0.y, f1.x, f1.y);
+              }
+            } else {
+              const uint32_t vw = vword(s, nb);
+              const uint8_t* q0 = smem + vaddr(vw, 0);
+              const uint8_t* q1 = smem + vaddr(vw, 1);
+              const uint8_t* q2 = smem + vaddr(vw, 2);
+              const uint8_t* q3 = smem + vaddr(vw, 3);
+              ah[n] = ba_h8(*reinterpret_cast<const uint32_t*>(q0), *reinterpret_cast<const uint32_t*>(q1),
+                            *reinterpret_cast<const uint32_t*>(q2), *reinterpret_cast<const uint32_t*>(q3));
+              if constexpr (PREC)
+                al[n] = ba_h8(*reinterpret_cast<const uint32_t*>(q0 + kBaLo), *reinterpret_cast<const uint32_t*>(q1 + kBaLo),
+                              *reinterpret_cast<const uint32_t*>(q2 + kBaLo), *reinterpret_cast<const uint32_t*>(q3 + kBaLo));
             }
-          } else {
-            const uint32_t vw = vword(s, nb);
-            const uint8_t* q0 = smem + vaddr(vw, 0);
-            const uint8_t* q1 = smem + vaddr(vw, 1);
-            const uint8_t* q2 = smem + vaddr(vw, 2);
-            const uint8_t* q3 = smem + vaddr(vw, 3);
-            ah = ba_h8(*reinterpret_cast<const uint32_t*>(q0), *reinterpret_cast<const uint32_t*>(q1),
-                       *reinterpret_cast<const uint32_t*>(q2), *reinterpret_cast<const uint32_t*>(q3));
-            if constexpr (PREC)
-              al = ba_h8(*reinterpret_cast<const uint32_t*>(q0 + kBaLo), *reinterpret_cast<const uint32_t*>(q1 + kBaLo),
-                         *reinterpret_cast<const uint32_t*>(q2 + kBaLo), *reinterpret_cast<const uint32_t*>(q3 + kBaLo));
           }
 #pragma unroll
-          for (int j = 0; j < NGR; ++j) {
-            o[j][nb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, bh[j][s], o[j][nb], 0, 0, 0);
-            if constexpr (PREC) {
-              o[j][nb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, bl[j][s], o[j][nb], 0, 0, 0);
-              o[j][nb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(al, bh[j][s], o[j][nb], 0, 0, 0);
-            }
-          }
+          for (int p = 0; p < (PREC ? 3 : 1); ++p)
+#pragma unroll
+            for (int n = 0; n < VN; ++n)
+#pragma unroll
+              for (int j = 0; j < NGR; ++j)
+                o[j][n0 + n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p == 2 ? al[PREC ? n : 0] : ah[n],
+                                                                      p == 1 ? bl[PREC ? j : 0][s] : bh[j][s],
+                                                                      o[j][n0 + n], 0, 0, 0);
         }
       }
     };
 
-    // two buffers, one tile ahead: the other waves of the SIMD cover the rest
+    // Two buffers, one tile ahead, the SIMD's other wave covering the rest; single tokens of fp32 /
+    // fp16 queries, whose tiles take longer, gain by a third (91 -> 87 us; bf16: 67 -> 69 us).
+    constexpr bool THREE = PREC && RW < 16;
     Tile r0, r1;
     if (nw > 0) load(0, r0);
+    if constexpr (THREE) {
+      if (nw > 0) load(1, r1);
+    }
     if (!built) {  // while the first tile is on its way
-      ba_build_tables<VB, PREC, WAVES>(a, smem);
+      ba_build_tables<VB, PREC>(a, smem);
       built = true;
     }
     if (nw > 0) {
       int i = 0;
-      for (; i + 1 < nw; i += 2) {
-        load(i + 1, r1);
-        compute(i, r0);
-        load(i + 2, r0);
-        compute(i + 1, r1);
+      if constexpr (THREE) {
+        Tile r2;
+        for (; i + 2 < nw; i += 3) {
+          load(i + 2, r2);
+          compute(i, r0);
+          load(i + 3, r0);
+          compute(i + 1, r1);
+          load(i + 4, r1);
+          compute(i + 2, r2);
+        }
+        if (i < nw) compute(i, r0);
+        if (i + 1 < nw) compute(i + 1, r1);
+      } else {
+        for (; i + 1 < nw; i += 2) {
+          load(i + 1, r1);
+          compute(i, r0);
+          load(i + 2, r0);
+          compute(i + 1, r1);
+        }
+        if (i < nw) compute(i, r0);
       }
-      if (i < nw) compute(i, r0);
     }
 
     if (next) it = ln.items[++item];
@@ -679,11 +737,9 @@ __device__ __forceinline__ void ba_piece(const BaArgs& a, const BaLine& ln, uint
 
 // Line 0 alone (PAIR: line 1, whose items hold many rows, before it: a wave goes on with its
 // piece of the sequences' line while others still read prefixes).
-template <int VB, bool SUB, bool PREC, int RW, int NGR, bool WIDE, bool PAIR>
-__global__ __launch_bounds__(64 * ba_waves(PREC, RW, NGR, PAIR), ba_waves(PREC, RW, NGR, PAIR) / 4)
-void batch_attn_kernel(BaArgs a) {
-  constexpr int WAVES = ba_waves(PREC, RW, NGR, PAIR);
-  __shared__ __attribute__((aligned(16))) uint8_t smem[kBaNorms + WAVES * 512];
+template <int VB, bool SUB, bool PREC, int RW, int NGR, bool WIDE, bool PAIR, bool MODS>
+__global__ __launch_bounds__(64 * kBaWaves, kBaWaves / 4) void batch_attn_kernel(BaArgs a) {
+  __shared__ __attribute__((aligned(16))) uint8_t smem[kBaNorms + kBaWaves * 512];
   // Neighbouring pieces on one XCD (workgroup w runs on XCD w % 8): rows of one prefix read the
   // same tiles there, and adjacent KV heads of a 16-token block share lines of norms.  Few
   // pieces spread over the workgroups.
@@ -693,18 +749,23 @@ void batch_attn_kernel(BaArgs a) {
   if (a.line[0].work[blk] < 0 && !(PAIR && a.line[1].work[blk] >= 0)) return;
   const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)) * (int)grid + (int)blk;
   bool built = false;
-  if constexpr (PAIR) ba_piece<VB, SUB, PREC, 16, ba_groups(PREC, true), WIDE, WAVES>(a, a.line[1], smem, w, built);
-  ba_piece<VB, SUB, PREC, RW, NGR, WIDE, WAVES>(a, a.line[0], smem, w, built);
-  if (!built) ba_build_tables<VB, PREC, WAVES>(a, smem);
+  if constexpr (PAIR) ba_piece<VB, SUB, PREC, 16, ba_groups(PREC, true), WIDE, MODS>(a, a.line[1], smem, w, built);
+  ba_piece<VB, SUB, PREC, RW, NGR, WIDE, MODS>(a, a.line[0], smem, w, built);
+  if (!built) ba_build_tables<VB, PREC>(a, smem);
 }
 
 template <int VB, bool SUB, bool PREC, bool WIDE, bool PAIR>
 void ba_launch_kind(const BaArgs& a, int rw, int groups, unsigned grid, hipStream_t st) {
-  const dim3 gr(grid), bl(64 * ba_waves(PREC, rw, groups, PAIR));
-  if (groups > 1) hipLaunchKernelGGL((batch_attn_kernel<VB, SUB, PREC, 16, ba_groups(PREC, PAIR), WIDE, PAIR>), gr, bl, 0, st, a);
-  else if (rw == 16) hipLaunchKernelGGL((batch_attn_kernel<VB, SUB, PREC, 16, 1, WIDE, PAIR>), gr, bl, 0, st, a);
-  else if (rw == 8) hipLaunchKernelGGL((batch_attn_kernel<VB, SUB, PREC, 8, 1, WIDE, PAIR>), gr, bl, 0, st, a);
-  else hipLaunchKernelGGL((batch_attn_kernel<VB, SUB, PREC, 4, 1, WIDE, PAIR>), gr, bl, 0, st, a);
+  const dim3 gr(grid), bl(64 * kBaWaves);
+  // Kernels of many rows come without the code of caps and biases too, whose registers they miss:
+  // causal prompts 412 -> 391 us.
+  constexpr int N = ba_groups(PREC, PAIR);
+  const bool mods = a.cap2 != 0.f || a.slopes;
+  if (groups > 1 && mods) hipLaunchKernelGGL((batch_attn_kernel<VB, SUB, PREC, 16, N, WIDE, PAIR, true>), gr, bl, 0, st, a);
+  else if (groups > 1) hipLaunchKernelGGL((batch_attn_kernel<VB, SUB, PREC, 16, N, WIDE, PAIR, false>), gr, bl, 0, st, a);
+  else if (rw == 16) hipLaunchKernelGGL((batch_attn_kernel<VB, SUB, PREC, 16, 1, WIDE, PAIR, true>), gr, bl, 0, st, a);
+  else if (rw == 8) hipLaunchKernelGGL((batch_attn_kernel<VB, SUB, PREC, 8, 1, WIDE, PAIR, true>), gr, bl, 0, st, a);
+  else hipLaunchKernelGGL((batch_attn_kernel<VB, SUB, PREC, 4, 1, WIDE, PAIR, true>), gr, bl, 0, st, a);
 }
 
 template <int VB, bool SUB, bool PAIR>
