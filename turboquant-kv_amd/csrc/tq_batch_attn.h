@@ -50,7 +50,7 @@ namespace tq {
 // Waves of a workgroup (one per CU: the tables fill its LDS).  256 registers a wave; 12 waves of 168
 // were no faster (48 sequences of up to 32k tokens: 89 and 91 us) and leave more to be joined.
 constexpr int kBaWaves = 8;
-constexpr int kBaMaxSegs = 8191;  // sequences or groups of a call: the preparing kernel's LDS
+constexpr int kBaMaxSegs = 8192;  // sequences or groups of a call: the preparing kernel's LDS
 constexpr int kBaQueryTop = 14;   // rotated queries are scaled to at most 2^14 (fp16's range ends at 2^16)
 constexpr int kBaOver = 3;        // an (item, head)'s cost besides its tiles, in tiles
 // Groups of 16 rows that a wave takes where rows abound.  Three share a tile's lookups best where
@@ -89,7 +89,7 @@ struct BaLine {
   int32_t waves;
   int32_t rows;        // R
   float* slots;        // [waves][2][ba_slot_floats(R)]
-  float* row_sums;     // [n_tokens * hq][64]
+  float* row_sums;     // [n_tokens * hq][64] (not where waves write results)
   float* row_stats;    // [n_tokens * hq][2]
 };
 // A token's visible positions, its own, and its sequence (B: behind the last).

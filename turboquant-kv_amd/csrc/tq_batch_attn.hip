@@ -11,6 +11,7 @@ namespace {
 constexpr int kPrepThreads = 512;
 constexpr int kPrepWaves = kPrepThreads / 64;
 constexpr int kPrepStarts = 2048;  // items' places kept in LDS
+constexpr float kBaBalance = 64.f;  // see ba_lay_out's pieces
 
 // ---------------------------------------------------------------------------- preparation
 
@@ -103,6 +104,7 @@ __device__ __forceinline__ void ba_lay_out(const BaArgs& a, int32_t* base_s, int
   // (starts that do not ascend could make more items than there is room for)
   const int n_items = min(base_s[nseg], ln.max_items);
   int64_t place = 0;
+  int most = 0;  // tiles of an item
   for (int i0 = 0; i0 < n_items; i0 += kPrepThreads) {
     const int i = i0 + tid;
     int64_t cost = 0, all;
@@ -132,6 +134,7 @@ __device__ __forceinline__ void ba_lay_out(const BaArgs& a, int32_t* base_s, int
       it.t0 = hi > lo ? (int)(lo >> 6) : 0;
       it.nt = hi > lo ? (int)((hi + 63) >> 6) - it.t0 : 0;
       cost = (int64_t)(it.nt + kBaOver) * a.hkv;
+      most = max(most, it.nt);
     }
     const int64_t at = prep_scan(cost, part, &all);
     if (i < n_items) {
@@ -141,8 +144,19 @@ __device__ __forceinline__ void ba_lay_out(const BaArgs& a, int32_t* base_s, int
     }
     place += all;
   }
-  // Equal pieces, of two tiles at least: a single one would double what is to be joined.
-  const int64_t chunk = max<int64_t>(2, ba_div(place + ln.waves - 1, ln.waves));
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) most = max(most, __shfl_xor(most, o, 64));
+  __syncthreads();
+  if ((tid & 63) == 0) part[tid >> 6] = most;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kPrepWaves; ++w) most = max(most, (int)part[w]);
+  // Equal pieces, of two tiles at least: a single one would double what is to be joined.  An (item,
+  // head) of n tiles in k pieces costs its waves about 0.6 us for each of n / k tiles, and those
+  // who join it 0.01 us for each of k pieces: the sum is least at about sqrt(n / 64) tiles a piece
+  // (one token of 8 heads over 524288: 18 + 11 us where two tiles a piece took 14 + 14).
+  const int64_t least = max(2, (int)ceilf(sqrtf((float)most * (1.f / kBaBalance))));
+  const int64_t chunk = max<int64_t>(least, ba_div(place + ln.waves - 1, ln.waves));
   if (tid == 0) *ln.head = BaHead{chunk, place, n_items, 0};
   // The item that each wave's piece begins in: a wave per item fills its waves' entries, or,
   // where items abound, each entry searches for its own.
@@ -412,198 +426,262 @@ __device__ __forceinline__ BaFrom ba_from(const BaArgs& a, const BaLine& ln, int
   return f;
 }
 
-constexpr int kJoinWaves = 4;
+constexpr int kJoinAhead = 4;   // sources a wave asks for at once
+constexpr int kTailBlocks = 32;
 
-// 16 rows (a token's head each) per workgroup: a row's sums come from its sequence's line and,
-// with groups, from its group's.  The waves take a row's sources in turn, join theirs, then
-// wave ob rotates dims 16 ob .. of the whole back by R_v.  A source is 264 bytes of a row;
-// latency bounds it (a few microseconds).
-__global__ __launch_bounds__(64 * kJoinWaves) void batch_join_kernel(BaArgs a) {
+// ROWS = 16 rows (a token's head each) per workgroup, lane (c, g) dims 16 nb + 4 g .. of row c.
+// WAVES waves take a row's sources in turn and join theirs, then share the rotation of the whole
+// back by R_v.  A source is 264 bytes of a row; latency bounds a few of them (5 us with the launch).
+// ROWS = 1: a workgroup per row, whose columns c take sources in turn too: a CU reads what others
+// wrote at about 40 GB/s, so few rows of many pieces need more CUs.
+//   kJoinRows: any 16 neighbouring rows; a row's sources are its sequence's line's and, with
+//   groups, its group's.
+//   Where waves write the results of whole items themselves, the last kTailBlocks workgroups
+//   write the rows behind the last sequence, and
+//   kJoinItems: workgroup (item, head, j) joins group (ROWS = 1: row) j of the (item, head) if
+//   it was cut;
+//   kJoinBorders: workgroup (w, j) joins group j of the (item, head) that the border before
+//   wave w's piece cuts, if it is that one's first border.
+enum { kJoinRows, kJoinItems, kJoinBorders };
+template <int BY, int WAVES, int ROWS>
+__global__ __launch_bounds__(64 * WAVES) void batch_join_kernel(BaArgs a) {
 #pragma clang fp contract(off)
-  __shared__ __attribute__((aligned(16))) float sums_s[kJoinWaves][16][68];
-  __shared__ float stat_s[kJoinWaves][16][2];
+  __shared__ __attribute__((aligned(16))) float sums_s[WAVES][16][68];
+  __shared__ float stat_s[WAVES][16][2];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, g = lane >> 4;
-  const int64_t n_rows = (int64_t)a.n_tokens * a.hq, r0 = (int64_t)blockIdx.x * 16;
-  const int64_t rowid = min(r0 + c, n_rows - 1);
-  const int tok = (int)ba_div(rowid, a.hq), qh = (int)(rowid - (int64_t)tok * a.hq);
-  const int h = qh / a.G, gq = qh - h * a.G;
-  // R_v's operands of this wave's dims, wanted last
-  ba_v8h rv[2][2];
+  const BaLine& ln0 = a.line[0];
+  int tok, qh;
+  int64_t rowid;
+  bool live, known = true;  // the lane's row exists; it belongs to a sequence
+  BaFrom s{}, p{};          // sources in lines 0 and 1
+  if constexpr (BY != kJoinRows) {
+    const int groups = ln0.rows / ROWS;
+    const int u = (int)(blockIdx.x / (unsigned)groups), j = (int)(blockIdx.x % (unsigned)groups);
+    const unsigned tail = gridDim.x - kTailBlocks;
+    if (blockIdx.x >= tail) {
+      const int first = a.B > 0 ? ba_qs(a, a.B) : 0, head = a.B > 0 ? ba_qs(a, 0) : 0;
+      const int64_t n = (int64_t)(a.n_tokens - first + head) * a.hq;
+      constexpr int kRows = 4 * WAVES;
+      for (int64_t i = (int64_t)(blockIdx.x - tail) * kRows + (tid >> 4); i < n;
+           i += kTailBlocks * kRows) {
+        const int t = (int)ba_div(i, a.hq);
+        tok = t < head ? t : first + t - head;
+        qh = (int)(i - (int64_t)t * a.hq);
+        if (a.zero_tail) ba_store(a, tok, qh, 4 * c, (ba_v4f){0.f, 0.f, 0.f, 0.f});
+        if (a.lse && c == 0) a.lse[(int64_t)tok * a.hq + qh] = -INFINITY;
+      }
+      return;
+    }
+    const BaHead hd = *ln0.head;
+    int i, h;
+    if constexpr (BY == kJoinItems) {
+      i = u / a.hkv;
+      h = u - i * a.hkv;
+      if (i >= hd.n_items) return;
+    } else {
+      if ((u + 1) * hd.chunk >= hd.total) return;
+      i = ln0.work[u + 1];
+    }
+    const BaItem it = ln0.items[i];
+    const int64_t cost = it.nt + kBaOver;
+    if constexpr (BY == kJoinBorders) h = (int)ba_div((u + 1) * hd.chunk - it.start, cost);
+    const int64_t start = it.start + h * cost;
+    s.w0 = ba_div(start + kBaOver, hd.chunk);
+    const int64_t w1 = ba_div(start + cost - 1, hd.chunk);
+    if (s.w0 == w1 || it.nt == 0 || it.row0 + ROWS * j >= it.nrows || (BY == kJoinBorders && u != (int)s.w0)) return;
+    s.count = (int)(w1 - s.w0) + 1;
+    s.row = ROWS * j + (ROWS > 1 ? c : 0);
+    live = it.row0 + s.row < it.nrows;
+    const int row = min(it.row0 + s.row, it.nrows - 1), ti = row / a.G;
+    tok = it.tok0 + ti;
+    qh = h * a.G + (row - ti * a.G);
+    rowid = (int64_t)tok * a.hq + qh;
+  } else {
+    const int64_t n_rows = (int64_t)a.n_tokens * a.hq, r0 = (int64_t)blockIdx.x * ROWS;
+    rowid = min(r0 + (ROWS > 1 ? c : 0), n_rows - 1);
+    live = r0 + (ROWS > 1 ? c : 0) < n_rows;
+    tok = (int)ba_div(rowid, a.hq);
+    qh = (int)(rowid - (int64_t)tok * a.hq);
+  }
+  // R_v's operands of this wave's dims (wave ob: 16 ob ..; one wave: all), wanted last
+  constexpr int OBS = 4 / WAVES;
+  ba_v8h rv[OBS][2][2];
+  auto load_rv = [&] {
 #pragma unroll
-  for (int part = 0; part < 2; ++part)
+    for (int ob = 0; ob < OBS; ++ob)
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
-      rv[part][s] = reinterpret_cast<const ba_v8h*>(a.vrot16)[(part * 8 + wave * 2 + s) * 64 + lane];
-  const BaToken t = a.tokens[tok];
-  BaFrom s{}, p{};
-  if (t.seq < a.B) {
-    s = ba_from(a, a.line[0], t.seq, (int64_t)(tok - ba_qs(a, t.seq)) * a.G + gq, h);
-    if (a.n_groups > 0) {
-      const int gi = ba_last(a.n_groups, t.seq, [&](int i) { return a.group_start[i]; });
-      const int b0 = a.group_start[gi], b1 = min(a.group_start[gi + 1], a.B);
-      if (b0 >= 0 && t.seq >= b0 && t.seq < b1 && a.shared[gi] > 0 && a.cap > 0)
-        p = ba_from(a, a.line[1], gi, (int64_t)(tok - ba_qs(a, b0)) * a.G + gq, h);
+      for (int part = 0; part < 2; ++part)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          rv[ob][part][k] = reinterpret_cast<const ba_v8h*>(a.vrot16)[(part * 8 + (wave * OBS + ob) * 2 + k) * 64 + lane];
+  };
+  if constexpr (WAVES > 1) load_rv();
+  if constexpr (BY == kJoinRows) {
+    const int h = qh / a.G, gq = qh - h * a.G;
+    const BaToken t = a.tokens[tok];
+    known = t.seq < a.B;
+    if (known) {
+      s = ba_from(a, ln0, t.seq, (int64_t)(tok - ba_qs(a, t.seq)) * a.G + gq, h);
+      if (a.n_groups > 0) {
+        const int gi = ba_last(a.n_groups, t.seq, [&](int i) { return a.group_start[i]; });
+        const int b0 = a.group_start[gi], b1 = min(a.group_start[gi + 1], a.B);
+        if (b0 >= 0 && t.seq >= b0 && t.seq < b1 && a.shared[gi] > 0 && a.cap > 0)
+          p = ba_from(a, a.line[1], gi, (int64_t)(tok - ba_qs(a, b0)) * a.G + gq, h);
+      }
     }
   }
   const int ns = s.count, np = p.count;
   int most = ns + np;
 #pragma unroll
   for (int o = 8; o >= 1; o >>= 1) most = max(most, __shfl_xor(most, o, 64));
+  most = __builtin_amdgcn_readfirstlane(most);
 
+  struct Source {
+    float m, l;
+    ba_v4f v[4];
+  };
+  // source i of the lane's row (behind its last: nothing)
+  auto load = [&](int i, Source& x) {
+    const bool mine = i < ns, any = i < ns + np;
+    const BaFrom& f = mine ? s : p;
+    const BaLine& ln = BY != kJoinRows || mine || !any ? ln0 : a.line[1];
+    const int k = !any ? 0 : mine ? i : i - ns;
+    // the wave with the item's first tile kept it in slot 1
+    const float* slot = ln.slots + (any ? (f.w0 + k) * 2 + (k == 0) : 0) * ba_slot_floats(ln.rows);
+    const bool by_row = BY == kJoinRows && any && f.by_row;
+    const int row = any ? f.row : 0;
+    const float* sums = by_row ? ln.row_sums + rowid * 64 : slot + row * 64;
+    const float* st = by_row ? ln.row_stats + rowid * 2 : slot + ln.rows * 64 + row * 2;
+    x.m = st[0];
+    x.l = st[1];
+#pragma unroll
+    for (int nb = 0; nb < 4; ++nb) x.v[nb] = *reinterpret_cast<const ba_v4f*>(sums + 16 * nb + 4 * g);
+    if (!any) {  // (what was read may be NaN)
+      x.m = -INFINITY;
+      x.l = 0.f;
+#pragma unroll
+      for (int nb = 0; nb < 4; ++nb) x.v[nb] = (ba_v4f){0.f, 0.f, 0.f, 0.f};
+    }
+  };
   float m = -INFINITY, l = 0.f;
   ba_v4f o4[4];
 #pragma unroll
   for (int nb = 0; nb < 4; ++nb) o4[nb] = (ba_v4f){0.f, 0.f, 0.f, 0.f};
-  for (int i = wave; i < most; i += kJoinWaves) {
-    if (i >= ns + np) continue;
-    const bool mine = i < ns;
-    const float *sums, *st;
-    auto source = [&](const BaLine& ln, const BaFrom& f, int k) {
-      // the wave with the item's first tile kept it in slot 1
-      const float* slot = ln.slots + ((f.w0 + k) * 2 + (k == 0)) * ba_slot_floats(ln.rows);
-      sums = f.by_row ? ln.row_sums + rowid * 64 : slot + f.row * 64;
-      st = f.by_row ? ln.row_stats + rowid * 2 : slot + ln.rows * 64 + f.row * 2;
-    };
-    if (mine) source(a.line[0], s, i);
-    else source(a.line[1], p, i - ns);
-    const float mi = st[0], li = st[1];
-    const float mn = fmaxf(m, mi), ms = mn == -INFINITY ? 0.f : mn;
-    const float fa = __builtin_amdgcn_exp2f(m - ms), fb = __builtin_amdgcn_exp2f(mi - ms);
+  auto add = [&](const Source& x) {
+    const float mn = fmaxf(m, x.m), ms = mn == -INFINITY ? 0.f : mn;
+    const float fa = __builtin_amdgcn_exp2f(m - ms), fb = __builtin_amdgcn_exp2f(x.m - ms);
     m = mn;
-    l = l * fa + li * fb;
+    l = l * fa + x.l * fb;
 #pragma unroll
-    for (int nb = 0; nb < 4; ++nb)
-      o4[nb] = o4[nb] * fa + *reinterpret_cast<const ba_v4f*>(sums + 16 * nb + 4 * g) * fb;
+    for (int nb = 0; nb < 4; ++nb) o4[nb] = o4[nb] * fa + x.v[nb] * fb;
+  };
+  constexpr int STEP = WAVES * (16 / ROWS);  // sources taken at once
+  const int first = ROWS > 1 ? wave : 16 * wave + c;
+  if (most <= STEP) {
+    if (first < most) {
+      Source x;
+      load(first, x);
+      add(x);
+    }
+  } else {
+    constexpr int AHEAD = WAVES > 1 ? kJoinAhead : 2;
+    for (int i = 0; i < most; i += AHEAD * STEP) {
+      Source x[AHEAD];
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) load(i + first + u * STEP, x[u]);
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) add(x[u]);
+    }
   }
+  if constexpr (ROWS == 1) {  // over the columns
+    float mn = m;
 #pragma unroll
-  for (int nb = 0; nb < 4; ++nb) *reinterpret_cast<ba_v4f*>(&sums_s[wave][c][16 * nb + 4 * g]) = o4[nb];
-  if (g == 0) {
-    stat_s[wave][c][0] = m;
-    stat_s[wave][c][1] = l;
+    for (int o = 1; o < 16; o <<= 1) mn = fmaxf(mn, __shfl_xor(mn, o, 64));
+    const float f = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+    m = mn;
+    l *= f;
+#pragma unroll
+    for (int nb = 0; nb < 4; ++nb) o4[nb] *= f;
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) {
+      l += __shfl_xor(l, o, 64);
+#pragma unroll
+      for (int nb = 0; nb < 4; ++nb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o4[nb][r] += __shfl_xor(o4[nb][r], o, 64);
+    }
   }
-  __syncthreads();
-  float M = -INFINITY, L = 0.f, f[kJoinWaves];
+  if constexpr (WAVES > 1) {
 #pragma unroll
-  for (int w = 0; w < kJoinWaves; ++w) M = fmaxf(M, stat_s[w][c][0]);
-  const float Ms = M == -INFINITY ? 0.f : M;
+    for (int nb = 0; nb < 4; ++nb) *reinterpret_cast<ba_v4f*>(&sums_s[wave][c][16 * nb + 4 * g]) = o4[nb];
+    if (g == 0) {
+      stat_s[wave][c][0] = m;
+      stat_s[wave][c][1] = l;
+    }
+    __syncthreads();
+    float f[WAVES];
+    m = -INFINITY;
 #pragma unroll
-  for (int w = 0; w < kJoinWaves; ++w) {
-    f[w] = __builtin_amdgcn_exp2f(stat_s[w][c][0] - Ms);
-    L += stat_s[w][c][1] * f[w];
+    for (int w = 0; w < WAVES; ++w) m = fmaxf(m, stat_s[w][c][0]);
+    const float ms = m == -INFINITY ? 0.f : m;
+    l = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      f[w] = __builtin_amdgcn_exp2f(stat_s[w][c][0] - ms);
+      l += stat_s[w][c][1] * f[w];
+    }
+#pragma unroll
+    for (int nb = 0; nb < 4; ++nb) {
+      o4[nb] = (ba_v4f){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) o4[nb] += *reinterpret_cast<const ba_v4f*>(&sums_s[w][c][16 * nb + 4 * g]) * f[w];
+    }
+  } else {
+    load_rv();
   }
-  // ba_rotate_back for one ob, into fp16's range by a power of two of the row
-  const float inv = L == 0.f ? 0.f : 1.f / L;
-  float x[16], xm = 0.f;
+  // ba_rotate_back for this wave's dims, into fp16's range by a power of two of the row
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  float xm = 0.f;
 #pragma unroll
   for (int nb = 0; nb < 4; ++nb) {
-    ba_v4f v = {0.f, 0.f, 0.f, 0.f};
+    o4[nb] *= inv;
 #pragma unroll
-    for (int w = 0; w < kJoinWaves; ++w) v += *reinterpret_cast<const ba_v4f*>(&sums_s[w][c][16 * nb + 4 * g]) * f[w];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      x[4 * nb + r] = v[r] * inv;
-      xm = fmaxf(xm, fabsf(x[4 * nb + r]));
-    }
+    for (int r = 0; r < 4; ++r) xm = fmaxf(xm, fabsf(o4[nb][r]));
   }
   xm = fmaxf(xm, __shfl_xor(xm, 16, 64));
   xm = fmaxf(xm, __shfl_xor(xm, 32, 64));
   const int e = ba_exponent(xm);
-  const float up = ldexpf(1.f, 4 - e);
+  const float up = ldexpf(1.f, 4 - e), down = ldexpf(1.f, e - 4);
   ba_v8h hi[2], lo[2];
 #pragma unroll
-  for (int s = 0; s < 2; ++s)
+  for (int k = 0; k < 2; ++k)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int u = 0; u < 8; ++u) {
       _Float16 hv, lv;
-      split_f16(x[8 * s + i] * up, hv, lv);
-      hi[s][i] = hv;
-      lo[s][i] = lv;
+      split_f16(o4[2 * k + (u >> 2)][u & 3] * up, hv, lv);
+      hi[k][u] = hv;
+      lo[k][u] = lv;
     }
   mfma_operand_fence(hi[0], hi[1], lo[0], lo[1]);
-  ba_v4f acc = {0.f, 0.f, 0.f, 0.f};
+  ba_v4f acc[OBS];
 #pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(rv[1][s], hi[s], acc, 0, 0, 0);
-    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(rv[0][s], lo[s], acc, 0, 0, 0);
-    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(rv[0][s], hi[s], acc, 0, 0, 0);
-  }
-  acc *= ldexpf(1.f, e - 4);
-  if (r0 + c >= n_rows) return;
-  if (t.seq < a.B || a.zero_tail) ba_store(a, tok, qh, 16 * wave + 4 * g, acc);
-  if (a.lse && wave == 0 && g == 0) a.lse[rowid] = ba_lse(M, L);
-}
-
-// Where waves write whole items themselves: workgroup (w, j) joins group j of the (item, head)
-// that the border before wave w's piece cuts, if it is that one's first border; the last
-// kTailBlocks workgroups write the rows behind the last sequence.  A wave rotates a quarter of the
-// dims; all four read the sums of the waves that took a part.
-constexpr int kTailBlocks = 32;
-template <bool PREC>
-__global__ __launch_bounds__(64) void batch_join_cut_kernel(BaArgs a) {
-#pragma clang fp contract(off)
-  const BaLine& ln = a.line[0];
-  const int lane = threadIdx.x, c = lane & 15, g = lane >> 4;
-  const int groups = ln.rows / 16;
-  const int w = (int)(blockIdx.x / (unsigned)groups) + 1, j = (int)(blockIdx.x % (unsigned)groups);
-  if (w >= ln.waves) {
-    const int first = a.B > 0 ? ba_qs(a, a.B) : 0, head = a.B > 0 ? ba_qs(a, 0) : 0;
-    const int64_t n = (int64_t)(a.n_tokens - first + head) * a.hq;
-    for (int64_t i = (int64_t)(blockIdx.x - (unsigned)(groups * (ln.waves - 1))) * 4 + g; i < n; i += kTailBlocks * 4) {
-      const int t = (int)ba_div(i, a.hq), qh = (int)(i - (int64_t)t * a.hq);
-      const int tok = t < head ? t : first + t - head;
-      if (a.zero_tail) ba_store(a, tok, qh, 4 * c, (ba_v4f){0.f, 0.f, 0.f, 0.f});
-      if (a.lse && c == 0) a.lse[(int64_t)tok * a.hq + qh] = -INFINITY;
+  for (int ob = 0; ob < OBS; ++ob) {
+    acc[ob] = (ba_v4f){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      acc[ob] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rv[ob][1][k], hi[k], acc[ob], 0, 0, 0);
+      acc[ob] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rv[ob][0][k], lo[k], acc[ob], 0, 0, 0);
+      acc[ob] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rv[ob][0][k], hi[k], acc[ob], 0, 0, 0);
     }
-    return;
+    acc[ob] *= down;
   }
-  const int64_t chunk = ln.head->chunk, p = w * chunk;
-  if (p >= ln.head->total) return;
-  const BaItem it = ln.items[ln.work[w]];
-  const int64_t cost = it.nt + kBaOver;
-  const int h = (int)ba_div(p - it.start, cost);
-  const int64_t start = it.start + h * cost;
-  const int64_t w0 = ba_div(start + kBaOver, chunk), w1 = ba_div(start + cost - 1, chunk);
-  const int row = it.row0 + 16 * j + c;
-  if (w0 == w1 || it.nt == 0 || w != (int)w0 + 1 || it.row0 + 16 * j >= it.nrows) return;
-  float m = -INFINITY, l = 0.f;
-  ba_v4f x[4], out[4];
+  if (!live || (ROWS == 1 && c > 0)) return;
+  if (known || a.zero_tail)
 #pragma unroll
-  for (int nb = 0; nb < 4; ++nb) x[nb] = (ba_v4f){0.f, 0.f, 0.f, 0.f};
-  for (int64_t k = w0; k <= w1; ++k) {
-    const float* slot = ln.slots + (k * 2 + (k == w0)) * ba_slot_floats(ln.rows);
-    const float* sums = slot + (16 * j + c) * 64;
-    const float* st = slot + ln.rows * 64 + (16 * j + c) * 2;
-    const float mi = st[0], li = st[1];
-    const float mn = fmaxf(m, mi), ms = mn == -INFINITY ? 0.f : mn;
-    const float fa = __builtin_amdgcn_exp2f(m - ms), fb = __builtin_amdgcn_exp2f(mi - ms);
-    m = mn;
-    l = l * fa + li * fb;
-#pragma unroll
-    for (int nb = 0; nb < 4; ++nb)
-      x[nb] = x[nb] * fa + *reinterpret_cast<const ba_v4f*>(sums + 16 * nb + 4 * g) * fb;
-  }
-  // into fp16's range by a power of two of the row
-  float xm = 0.f;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-  for (int nb = 0; nb < 4; ++nb) {
-    x[nb] *= inv;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) xm = fmaxf(xm, fabsf(x[nb][r]));
-  }
-  xm = fmaxf(xm, __shfl_xor(xm, 16, 64));
-  xm = fmaxf(xm, __shfl_xor(xm, 32, 64));
-  const int e = ba_exponent(xm);
-#pragma unroll
-  for (int nb = 0; nb < 4; ++nb) x[nb] *= ldexpf(1.f, 4 - e);
-  ba_rotate_back<PREC>(a.vrot16, x, lane, out);
-  if (row >= it.nrows) return;
-  const int ti = row / a.G, tok = it.tok0 + ti, qh = h * a.G + (row - ti * a.G);
-#pragma unroll
-  for (int ob = 0; ob < 4; ++ob) ba_store(a, tok, qh, 16 * ob + 4 * g, out[ob] * ldexpf(1.f, e - 4));
-  if (a.lse && g == 0) a.lse[(int64_t)tok * a.hq + qh] = ba_lse(m, l);
+    for (int ob = 0; ob < OBS; ++ob) ba_store(a, tok, qh, 16 * (wave * OBS + ob) + 4 * g, acc[ob]);
+  if (a.lse && wave == 0 && g == 0) a.lse[rowid] = ba_lse(m, l);
 }
 
 // --------------------------------------------------------------------------------- plans
@@ -611,6 +689,7 @@ __global__ __launch_bounds__(64) void batch_join_cut_kernel(BaArgs a) {
 // Which kernels a call runs, and its workspace.
 struct BaPlan {
   bool prec, pair;
+  bool direct;           // waves write the results of whole items
   int rw[2], groups[2];  // per line: rows of a group of columns, groups
   int64_t items[2];
   unsigned grid;
@@ -639,6 +718,7 @@ BaPlan ba_plan(tq_dtype q_dtype, int64_t n, int hq, int hkv, int64_t B, int64_t 
     const int64_t pieces = p.items[l] * hkv * (capacity / 64 + 1 + kBaOver);
     p.grid = std::max(p.grid, (unsigned)std::max<int64_t>(1, std::min(cus, pieces)));
   }
+  p.direct = !p.pair && p.groups[0] > 1;
   return p;
 }
 
@@ -669,6 +749,7 @@ size_t ba_place(const BaPlan& p, int64_t n, int hq, char* at, BaArgs* a) {
     ln.seg_item = reinterpret_cast<int32_t*>(take((p.segs[l] + 1) * 4));
     ln.work = reinterpret_cast<int32_t*>(take((size_t)ln.waves * 4));
     ln.slots = reinterpret_cast<float*>(take((size_t)ln.waves * 2 * ba_slot_floats(ln.rows) * 4));
+    if (p.direct) continue;  // whole items leave results, not sums
     ln.row_sums = reinterpret_cast<float*>(take(rows * 256));
     ln.row_stats = reinterpret_cast<float*>(take(rows * 8));
   }
@@ -690,6 +771,30 @@ void ba_run(int vbits, const BaArgs& a, const BaPlan& p, hipStream_t st) {
   if (vbits == 2) ba_run_bits<2>(a, p, st);
   else if (vbits == 3) ba_run_bits<3>(a, p, st);
   else ba_run_bits<4>(a, p, st);
+}
+
+template <int BY, int WAVES, int ROWS>
+void ba_join_by(const BaArgs& a, int64_t grid, hipStream_t st) {
+  hipLaunchKernelGGL((batch_join_kernel<BY, WAVES, ROWS>), dim3((unsigned)grid), dim3(64 * WAVES), 0, st, a);
+}
+
+// Few rows, whose pieces may be many, have a workgroup each (one token of 8 heads over 131072: 17.8 ->
+// 7.1 us; 48 tokens of 32 heads over 8192 fill the chip with 16 rows each: 6.4 us against 14.2).  Where waves wrote whole items themselves and there are as many (item, head)s as waves,
+// few of them lie in more than two pieces, and a wave joins each: 15 us for 4096-token prompts, 28
+// with four waves.
+void ba_join(const BaArgs& a, const BaPlan& p, hipStream_t st) {
+  const int64_t pairs = p.items[0] * a.hkv, R = a.line[0].rows;
+  const int64_t rows = (int64_t)a.n_tokens * a.hq, most = 2 * device_cu_count();
+  if (!a.direct) {
+    if (rows <= most) ba_join_by<kJoinRows, 4, 1>(a, rows, st);
+    else ba_join_by<kJoinRows, 4, 16>(a, (rows + 15) / 16, st);
+  } else if (pairs >= a.line[0].waves) {
+    ba_join_by<kJoinBorders, 1, 16>(a, (a.line[0].waves - 1) * (R / 16) + kTailBlocks, st);
+  } else if (rows <= most) {
+    ba_join_by<kJoinItems, 4, 1>(a, pairs * R + kTailBlocks, st);
+  } else {
+    ba_join_by<kJoinItems, 4, 16>(a, pairs * (R / 16) + kTailBlocks, st);
+  }
 }
 
 }  // namespace
@@ -726,8 +831,8 @@ int tq_attention_batch_paged_dl(const void* q, tq_dtype q_dtype, int32_t n_token
   TQ_REQUIRE(block_size >= 16 && (1 << bsl) == block_size,
              "decode-layout pools need a power-of-two block_size >= 16, got %d", block_size);
   TQ_REQUIRE(n_tokens >= 0 && n_seqs >= 0 && n_groups >= 0 && max_blocks >= 0 && num_blocks >= 0, "bad sizes");
-  TQ_REQUIRE(n_seqs < kBaMaxSegs && n_groups <= kBaMaxSegs, "a call takes at most %d sequences and %d groups, got %d and %d",
-             kBaMaxSegs - 1, kBaMaxSegs, n_seqs, n_groups);
+  TQ_REQUIRE(n_seqs <= kBaMaxSegs && n_groups <= kBaMaxSegs, "a call takes at most %d sequences and groups, got %d and %d",
+             kBaMaxSegs, n_seqs, n_groups);
   TQ_REQUIRE(num_blocks <= (int64_t)UINT_MAX, "too many blocks");
   TQ_REQUIRE(table_stride >= max_blocks, "table rows of %d entries overlap at a stride of %lld", max_blocks,
              (long long)table_stride);
@@ -740,7 +845,8 @@ int tq_attention_batch_paged_dl(const void* q, tq_dtype q_dtype, int32_t n_token
   TQ_REQUIRE(q_stride >= row_elems && out_stride >= row_elems, "rows of %lld elements overlap", (long long)row_elems);
   const tq_score_variant none{};
   const tq_score_variant& v = variant ? *variant : none;
-  TQ_REQUIRE(v.softcap >= 0.f && v.softcap < INFINITY, "softcap must be finite and not negative, got %g", v.softcap);
+  TQ_REQUIRE(v.softcap == 0.f || (v.softcap >= 1e-30f && v.softcap <= 1e30f),
+             "softcap must be 0 or in [1e-30, 1e30], got %g", v.softcap);
   TQ_REQUIRE(v.window >= 0, "window must not be negative, got %d", v.window);
   TQ_REQUIRE(q && out && (n_seqs == 0 || (query_start_loc && seq_lens)) && kcentroids && vcentroids && krotation &&
                  vrotation && (n_groups == 0 || (group_start_loc && shared_lens)),
@@ -784,7 +890,7 @@ int tq_attention_batch_paged_dl(const void* q, tq_dtype q_dtype, int32_t n_token
   hipStream_t st = as_stream(stream);
   const int lines = n_groups > 0 ? 2 : 1;
   const int64_t qrows = (int64_t)n_tokens * hq;
-  a.direct = n_groups == 0 && p.groups[0] > 1;
+  a.direct = p.direct;
   // waves of several rounds share R_k's parts: about two workgroups a CU at the most
   const int64_t rot = std::min<int64_t>((qrows + 16 * kPrepWaves - 1) / (16 * kPrepWaves), 2 * device_cu_count());
   const dim3 prep((unsigned)(lines + 1 + rot)), pthreads(kPrepThreads);
@@ -794,13 +900,7 @@ int tq_attention_batch_paged_dl(const void* q, tq_dtype q_dtype, int32_t n_token
   TQ_LAUNCH_CHECK("batch_prep_kernel");
   ba_run(vbits, a, p, st);
   TQ_LAUNCH_CHECK("batch_attn_kernel");
-  if (a.direct) {
-    const dim3 cut((unsigned)((a.line[0].waves - 1) * p.groups[0] + kTailBlocks));
-    if (p.prec) hipLaunchKernelGGL((batch_join_cut_kernel<true>), cut, dim3(64), 0, st, a);
-    else hipLaunchKernelGGL((batch_join_cut_kernel<false>), cut, dim3(64), 0, st, a);
-  } else {
-    hipLaunchKernelGGL(batch_join_kernel, dim3((unsigned)((qrows + 15) / 16)), dim3(64 * kJoinWaves), 0, st, a);
-  }
+  ba_join(a, p, st);
   TQ_LAUNCH_CHECK("batch_join_kernel");
   return TQ_OK;
 }
