@@ -1225,7 +1225,9 @@ void prefill_attention_paged_dl_out(
 
 at::Tensor int32c(const at::Tensor& t, const at::Device& dev, const char* name) {
   TORCH_CHECK(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, name, " must hold 32- or 64-bit integers");
-  return t.to(dev, at::kInt).contiguous();
+  // (64-bit values past 32 bits, as of a mask that hides everything, keep their meaning)
+  if (t.scalar_type() == at::kLong) return t.to(dev).clamp(INT32_MIN, INT32_MAX).to(at::kInt).contiguous();
+  return t.to(dev).contiguous();
 }
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> paged_batch_plan(
@@ -1354,7 +1356,7 @@ std::tuple<at::Tensor, at::Tensor> attention_batch(
               "decode layout: 4-bit keys (16 centroids) and 2^VB value centroids for the pool's "
               "VB-bit value tiles");
   TORCH_CHECK(Rk.numel() == d * d && Rv.numel() == d * d, "rotations must be [d, d]");
-  TORCH_CHECK(softcap >= 0 && std::isfinite(softcap), "softcap must be finite and not negative, got ", softcap);
+  TORCH_CHECK(softcap == 0 || (softcap >= 1e-30 && softcap <= 1e30), "softcap must be 0 or in [1e-30, 1e30], got ", softcap);
   TORCH_CHECK(window >= 0, "window must not be negative, got ", window);
   TORCH_CHECK(n <= INT32_MAX && B < INT32_MAX && Hq <= INT32_MAX && bt.size(1) <= INT32_MAX, "too many tokens");
   tq_score_variant v{};

@@ -313,8 +313,9 @@ def attention_batch_paged_dl(q, kpairs_pool, knorm_pool, vtile_pool, vnorm_pool,
 
     -> [num_tokens, Hq, 64] in q's dtype, zeros for rows that see nothing; with return_lse also
     the [num_tokens, Hq] float32 log-sum-exp of the scores (-inf there).  Rows behind the last
-    sequence are zeros, or keep their values in a given `out` (which must not share q's memory).
-    For inference: no gradient flows through it."""
+    sequence are zeros, or keep their values in a given `out` (which may be q: all queries are
+    read before a row is written).  At most 8192 sequences.  softcap is 0 or in [1e-30, 1e30].
+    64-bit lengths and masks saturate at 32 bits.  For inference: no gradient flows through it."""
     return _attention_batch(q, (kpairs_pool, knorm_pool, vtile_pool, vnorm_pool), block_tables,
                             query_start_loc, seq_lens, (None, None),
                             (kcentroids, vcentroids, krotation, vrotation), scale, softcap, alibi_slopes,

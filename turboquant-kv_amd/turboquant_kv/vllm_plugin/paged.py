@@ -392,7 +392,7 @@ class PagedKVPools:
         output keeps its rows there).  Decode-layout pools: one call, no host copy of lengths."""
         v = variant if variant is not None else AttentionVariant()
         st = self.layers[layer]
-        q = q.to(self.device)
+        given, q = q, q.to(self.device)
         if v.alibi_slopes is not None and not v.alibi_slopes.is_cuda:
             v.alibi_slopes = v.alibi_slopes.to(self.device)  # once: later steps may be captured
         kw = dict(softcap=v.softcap, alibi_slopes=v.alibi_slopes, window=v.window,
@@ -400,10 +400,9 @@ class PagedKVPools:
         if "kp" in st:
             wide = q.dtype == torch.float64  # computed in float32, as the other paths do
             qc = q.float() if wide else q
-            # the kernels read q while they write: a result in its memory takes a copy
+            # (all queries are read before a row is written: the result may lie in their memory)
             direct = (output is not None and output.device == q.device and output.shape == q.shape
-                      and output.dtype == qc.dtype and not _shares_memory(output, q)
-                      and output.stride()[1:] == (q.shape[2], 1) and output.data_ptr() % 16 == 0
+                      and output.dtype == qc.dtype and output.stride()[1:] == (q.shape[2], 1) and output.data_ptr() % 16 == 0
                       and output.stride(0) >= q.shape[1] * q.shape[2]
                       and output.stride(0) * output.element_size() % 16 == 0)
             args = [qc, st["kp"], st["kn"], st["vt"], st["vn"], md.block_tables, md.query_start_loc,
@@ -417,12 +416,12 @@ class PagedKVPools:
             else:
                 res = ops.attention_batch_paged_dl(*args, *tail, **kw)
             if output is None or direct:
-                return res.to(q.dtype) if output is None else res
+                return res.to(given) if output is None else res
             # a few rows behind the last sequence keep the output's values
-            live = torch.arange(q.shape[0], device=q.device) < md.query_start_loc.to(q.device)[-1]
-            output.copy_(torch.where(live[:, None, None], res.to(output.dtype), output))
+            live = torch.arange(q.shape[0], device=output.device) < md.query_start_loc.to(output.device)[-1]
+            output.copy_(torch.where(live[:, None, None], res.to(output), output))
             return output
-        out = output if output is not None else torch.zeros_like(q)
+        out = output if output is not None else torch.zeros_like(given)
         qsl = md.query_start_loc_cpu or md.query_start_loc.tolist()
         lens = md.seq_lens_cpu or md.seq_lens.tolist()
         for b, T in enumerate(lens):
