@@ -63,6 +63,24 @@ at::Tensor workspace(size_t bytes, const at::Device& dev) {
   return at::empty({(int64_t)(bytes > 0 ? bytes : 1)}, at::TensorOptions().dtype(at::kByte).device(dev));
 }
 
+// Tensors of one dimension side by side in one allocation, for operators whose many small results
+// would cost more to allocate (1.3 us each) than to compute.
+struct Carved {
+  at::Tensor bytes;
+  int64_t used = 0;
+  Carved(int64_t n, const at::Device& dev) : bytes(workspace((size_t)n, dev)) {}
+  static int64_t room(int64_t n, int64_t esz) { return (n * esz + 63) / 64 * 64; }
+  at::Tensor take(int64_t n, at::ScalarType type) {
+    const int64_t esz = (int64_t)c10::elementSize(type);
+    auto t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(bytes.storage()), bytes.key_set(),
+                                                      c10::scalarTypeToTypeMeta(type));
+    t.unsafeGetTensorImpl()->set_storage_offset(bytes.storage_offset() + used / esz);
+    t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+    used += room(n, esz);
+    return t;
+  }
+};
+
 int64_t packed_width(int64_t bits, int64_t d) { return bits * ((d + 7) / 8); }
 
 // ------------------------------------------------------------ reference schemas
@@ -1255,10 +1273,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tenso
     TORCH_CHECK(free_start->numel() == 1, "free_start must hold one value");
     fs = int32c(*free_start, dev, "free_start");
   }
-  const auto i32 = at::TensorOptions().dtype(at::kInt).device(dev);
-  const auto i64 = i32.dtype(at::kLong);
-  auto qs = at::empty({R + 1}, i32), sl = at::empty({R}, i32), sm = at::empty({num_tokens}, i64);
-  auto pos = at::empty({num_tokens}, i64), tr = at::empty({num_tokens}, i32), used = at::empty({1}, i32);
+  Carved all(Carved::room(R + 1, 4) + Carved::room(R, 4) + 2 * Carved::room(num_tokens, 8) + Carved::room(num_tokens, 4) + 64,
+             dev);
+  auto qs = all.take(R + 1, at::kInt), sl = all.take(R, at::kInt), sm = all.take(num_tokens, at::kLong);
+  auto pos = all.take(num_tokens, at::kLong), tr = all.take(num_tokens, at::kInt), used = all.take(1, at::kInt);
   check_rc(tq_paged_batch_plan(nl.data_ptr<int32_t>(), cl.data_ptr<int32_t>(), (int32_t)R,
                                block_tables.data_ptr<int32_t>(), R <= 1 ? block_tables.size(1) : block_tables.stride(0),
                                (int32_t)block_tables.size(1), fb.data_ptr<int32_t>(), fb.numel(),
@@ -1282,8 +1300,9 @@ std::tuple<at::Tensor, at::Tensor> shared_prefix_groups(const at::Tensor& block_
   TORCH_CHECK(block_size >= 1 && block_size <= INT32_MAX, "block_size must be positive, got ", block_size);
   TORCH_CHECK(min_tokens >= 1 && min_tokens <= INT32_MAX, "min_tokens must be positive, got ", min_tokens);
   TORCH_CHECK(R <= INT32_MAX && bt.size(1) <= INT32_MAX, "too many requests or blocks");
-  auto starts = at::empty({R + 1}, bt.options()), shared = at::empty({R}, bt.options());
-  auto ws = workspace(tq_shared_prefix_groups_workspace_bytes((int32_t)R), dev);
+  const size_t wsb = tq_shared_prefix_groups_workspace_bytes((int32_t)R);
+  Carved all(Carved::room(R + 1, 4) + Carved::room(R, 4) + Carved::room((int64_t)wsb, 1), dev);
+  auto starts = all.take(R + 1, at::kInt), shared = all.take(R, at::kInt), ws = all.take((int64_t)wsb, at::kByte);
   check_rc(tq_shared_prefix_groups(bt.data_ptr<int32_t>(), bt.size(1), (int32_t)bt.size(1), cl.data_ptr<int32_t>(),
                                    (int32_t)R, (int32_t)block_size, (int32_t)min_tokens, starts.data_ptr<int32_t>(),
                                    shared.data_ptr<int32_t>(), ws.data_ptr(), ws.numel(), cur_stream(bt)));
