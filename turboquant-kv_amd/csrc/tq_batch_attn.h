@@ -63,7 +63,7 @@ constexpr int ba_slot_floats(int R) { return R * 66; }
 // A line of work as the preparing kernel lays it out.
 struct BaHead {
   int64_t chunk, total;  // places of a wave's piece, of the line
-  int32_t n_items, pad;
+  int32_t n_items, pieces;
 };
 struct BaItem {
   int64_t start;      // its first place (KV head h: + h * (nt + kBaOver))

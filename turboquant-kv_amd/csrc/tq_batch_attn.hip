@@ -157,7 +157,7 @@ __device__ __forceinline__ void ba_lay_out(const BaArgs& a, int32_t* base_s, int
   // (one token of 8 heads over 524288: 18 + 11 us where two tiles a piece took 14 + 14).
   const int64_t least = max(2, (int)ceilf(sqrtf((float)most * (1.f / kBaBalance))));
   const int64_t chunk = max<int64_t>(least, ba_div(place + ln.waves - 1, ln.waves));
-  if (tid == 0) *ln.head = BaHead{chunk, place, n_items, 0};
+  if (tid == 0) *ln.head = BaHead{chunk, place, n_items, (int)ba_div(place + chunk - 1, chunk)};
   // The item that each wave's piece begins in: a wave per item fills its waves' entries, or,
   // where items abound, each entry searches for its own.
   if (n_items <= 8 * kPrepWaves) {

@@ -745,12 +745,28 @@ __global__ __launch_bounds__(64 * kBaWaves, kBaWaves / 4) void batch_attn_kernel
   // pieces spread over the workgroups.
   const unsigned grid = gridDim.x;
   const unsigned blk = grid % 8 == 0 ? (blockIdx.x % 8) * (grid / 8) + blockIdx.x / 8 : blockIdx.x;
-  // (a workgroup's first piece: where it lies behind the line's end, all do)
-  if (a.line[0].work[blk] < 0 && !(PAIR && a.line[1].work[blk] >= 0)) return;
   const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)) * (int)grid + (int)blk;
   bool built = false;
-  if constexpr (PAIR) ba_piece<VB, SUB, PREC, 16, ba_groups(PREC, true), WIDE, MODS>(a, a.line[1], smem, w, built);
-  ba_piece<VB, SUB, PREC, RW, NGR, WIDE, MODS>(a, a.line[0], smem, w, built);
+  if constexpr (PAIR) {
+    // Where both lines' pieces are few, line 0's begin behind line 1's, so that no wave takes one
+    // of each: 16 requests over 2048 shared tokens 14.6 -> 11.5 us.
+    const int waves = a.line[0].waves;
+    const int n1 = a.line[1].head->pieces, n0 = a.line[0].head->pieces;
+    const int skip = n1 + n0 <= waves ? n1 : 0;
+    bool busy = false;
+#pragma unroll
+    for (int k = 0; k < kBaWaves; ++k) {
+      const int x = k * (int)grid + (int)blk;
+      busy |= x < n1 || x - skip < n0;
+    }
+    if (!busy) return;
+    ba_piece<VB, SUB, PREC, 16, ba_groups(PREC, true), WIDE, MODS>(a, a.line[1], smem, w, built);
+    ba_piece<VB, SUB, PREC, RW, NGR, WIDE, MODS>(a, a.line[0], smem, w < skip ? w + waves - skip : w - skip, built);
+  } else {
+    // (a workgroup's first piece: where it lies behind the line's end, all do)
+    if (a.line[0].work[blk] < 0) return;
+    ba_piece<VB, SUB, PREC, RW, NGR, WIDE, MODS>(a, a.line[0], smem, w, built);
+  }
   if (!built) ba_build_tables<VB, PREC>(a, smem);
 }
 
