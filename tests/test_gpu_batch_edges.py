@@ -218,3 +218,20 @@ def test_softcaps_out_of_range(softcap):
     with pytest.raises(RuntimeError, match="softcap"):
         ops.attention_batch_paged_dl(q, *P.args(), torch.zeros(1, 2, dtype=torch.int32, device=DEV), _ints([0, 1]), _ints([9]),
                                      *P.tables(), 0.125, softcap=softcap)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("new", [[1, 1], [30, 2]])
+def test_subnormal_queries_and_values(dt, new):
+    """Queries and value norms near the end of fp32: weights are equal to rounding, and results are
+    as small as the values, whose rows of about 2^-114 an fp32 subnormal's 2^-149 resolves to 2^-35."""
+    rs = np.random.RandomState(40)
+    P = Pools(32, 60, 2, 16, 2)
+    lens = [300, 170]
+    tab = _tables(rs, lens, 16, P.nb)
+    q = (torch.from_numpy(rs.randn(sum(new), 8, 64)).to(DEV) * 2.0 ** -122).to(DTYPES[dt])
+    small = P.vn * 2.0 ** -115
+    a = (torch.from_numpy(tab).to(DEV), _ints([0, new[0], sum(new)]), _ints(lens), *P.tables(), 0.125)
+    got, lse = ops.attention_batch_paged_dl(q, P.kp, P.kn, P.vt, small, *a, return_lse=True)
+    out, wl, size = want(P, q, tab, new, lens, 0.125)
+    check(got.double() * 2.0 ** 115, lse, (out, wl, size), dt)

@@ -357,7 +357,7 @@ __device__ __forceinline__ void ba_rotate_rows(const BaArgs& a, int64_t blk, int
       }
     qm = fmaxf(qm, __shfl_xor(qm, 16, 64));
     qm = fmaxf(qm, __shfl_xor(qm, 32, 64));
-    const int e = ba_exponent(qm);
+    const int e = max(ba_exponent(qm), -110);  // (2^(14 - e) is finite, its inverse normal)
     const float qsc = ldexpf(1.f, kBaQueryTop - e);
     ba_v8h hi[2], lo[2];
 #pragma unroll
@@ -652,7 +652,7 @@ __global__ __launch_bounds__(64 * WAVES) void batch_join_kernel(BaArgs a) {
   }
   xm = fmaxf(xm, __shfl_xor(xm, 16, 64));
   xm = fmaxf(xm, __shfl_xor(xm, 32, 64));
-  const int e = ba_exponent(xm);
+  const int e = max(ba_exponent(xm), -122);  // (2^(4 - e) is finite, its inverse normal)
   const float up = ldexpf(1.f, 4 - e), down = ldexpf(1.f, e - 4);
   ba_v8h hi[2], lo[2];
 #pragma unroll
