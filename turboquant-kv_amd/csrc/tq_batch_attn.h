@@ -1,5 +1,6 @@
 // tq_batch_attn.h -- attention of a ragged batch over decode-layout paged pools on gfx950:
-// the kernel (instantiated per value width by tq_batch_attn_v{2,3,4}.hip) and its schedule.
+// the kernel (tq_batch_attn_kernel.h, instantiated per value width and pool by
+// tq_batch_attn_{2,3,4}{t,s}.hip) and its schedule.
 //
 // Semantics.  Sequence b's new tokens are rows query_start[b] .. query_start[b + 1] - 1 of q,
 // at positions p = T_b - n_b + i of its T_b = seq_lens[b] tokens.  A token sees the positions
@@ -14,7 +15,9 @@
 // head) preceded by kBaOver places that stand for what it costs besides its tiles.  Wave w of
 // the grid takes the w-th of equal pieces of that line, whatever the lengths are: no wave waits
 // for another.  A wave that takes all of an (item, head) leaves its sums by row, one that takes
-// a part leaves them in a slot of its own; the combine kernel joins them and rotates the result.
+// a part leaves them in a slot of its own; the joining kernel adds them up and rotates the result.
+// Items of many rows are mostly one wave's: without groups that wave rotates and writes their
+// results itself, and only cut items are joined.
 // With groups, the shared prefixes are a second line whose items hold the rows of all the
 // group's sequences: each of their tiles is read once for R rows of the group.
 // A preparing kernel rotates the queries, finds every token's positions and lays the line out

@@ -779,16 +779,17 @@ void ba_join_by(const BaArgs& a, int64_t grid, hipStream_t st) {
 }
 
 // Few rows, whose pieces may be many, have a workgroup each (one token of 8 heads over 131072: 17.8 ->
-// 7.1 us; 48 tokens of 32 heads over 8192 fill the chip with 16 rows each: 6.4 us against 14.2).  Where waves wrote whole items themselves and there are as many (item, head)s as waves,
-// few of them lie in more than two pieces, and a wave joins each: 15 us for 4096-token prompts, 28
-// with four waves.
+// 7.1 us; 48 tokens of 32 heads over 8192 fill the chip with 16 rows each: 6.4 us against 14.2).
+// Where waves wrote whole items themselves and the waves are at most four to an (item, head), few
+// of those lie in many pieces, and a wave joins each: 15 us for 4096-token prompts where four waves
+// took 28, 9.7 against 12.0 for chunks of 512 over 12288.
 void ba_join(const BaArgs& a, const BaPlan& p, hipStream_t st) {
   const int64_t pairs = p.items[0] * a.hkv, R = a.line[0].rows;
   const int64_t rows = (int64_t)a.n_tokens * a.hq, most = 2 * device_cu_count();
   if (!a.direct) {
     if (rows <= most) ba_join_by<kJoinRows, 4, 1>(a, rows, st);
     else ba_join_by<kJoinRows, 4, 16>(a, (rows + 15) / 16, st);
-  } else if (pairs >= a.line[0].waves) {
+  } else if (pairs * 4 >= a.line[0].waves) {
     ba_join_by<kJoinBorders, 1, 16>(a, (a.line[0].waves - 1) * (R / 16) + kTailBlocks, st);
   } else if (rows <= most) {
     ba_join_by<kJoinItems, 4, 1>(a, pairs * R + kTailBlocks, st);
