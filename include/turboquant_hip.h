@@ -678,7 +678,8 @@ int tq_shared_prefix_groups(const int32_t* block_tables, int64_t table_stride, i
 
 /* How scores are changed and which positions a query sees (zeros and nulls: not at all). */
 typedef struct tq_score_variant {
-  float softcap;               /* scores become softcap * tanh(score / softcap); 0: off */
+  float softcap;               /* scores become softcap * tanh(score / softcap); 0: off; in
+                                  [1e-30, 1e30] */
   const float* alibi_slopes;   /* [hq]: + slope * (key position - query position) */
   int32_t window;              /* the last `window` positions, the query's own included; 0: all */
   const int32_t* prefix_lens;  /* [n_seqs]: all tokens of a sequence see its first prefix_lens */
@@ -705,6 +706,8 @@ typedef struct tq_score_variant {
  * Replaces the reference backend's attention (vllm_plugin/__init__.py:400), whose Impl takes
  * alibi_slopes, sliding_window and logits_soft_cap and applies none of them.
  * Positions past max_blocks * block_size hold no tokens; block ids are clamped into the pool.
+ * At most 8192 sequences and 8192 groups.  All queries are read before a row of out is written,
+ * so out may lie in q's memory.
  * workspace: tq_attention_batch_workspace_bytes(.., capacity = max_blocks * block_size) bytes,
  * 16-byte aligned; calls that may run at the same time need one each.
  */

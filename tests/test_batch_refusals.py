@@ -6,6 +6,7 @@ import ctypes
 import pytest
 
 import capi
+from turboquant_kv.vllm_plugin import AttentionVariant
 
 ADDR = 1 << 20  # an aligned address that no refused call looks at
 i32, i64, f32, ptr, size = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t
@@ -91,3 +92,9 @@ def test_workspaces_of_wrong_sizes_are_empty():
     fn.argtypes, fn.restype = [i32, i32, i32, i32, i32, i32, i64], size
     for n, hq, hkv, B, g, cap in ((0, 8, 2, 1, 0, 64), (3, 8, 3, 1, 0, 64), (3, 8, 0, 1, 0, 64), (3, 8, 2, -1, 0, 64), (3, 8, 2, 1, 0, -1)):
         assert fn(0, n, hq, hkv, B, g, cap) == 0
+
+
+@pytest.mark.parametrize("kw", [dict(softcap=-1.0), dict(softcap=float("nan")), dict(softcap=float("inf")), dict(window=-1)])
+def test_score_variants(kw):
+    with pytest.raises(ValueError):
+        AttentionVariant(**kw)

@@ -235,3 +235,26 @@ def test_subnormal_queries_and_values(dt, new):
     got, lse = ops.attention_batch_paged_dl(q, P.kp, P.kn, P.vt, small, *a, return_lse=True)
     out, wl, size = want(P, q, tab, new, lens, 0.125)
     check(got.double() * 2.0 ** 115, lse, (out, wl, size), dt)
+
+
+@pytest.mark.parametrize("inference", [False, True])
+def test_small_results_are_tensors_of_their_own(inference):
+    """A plan's and the groups' results come from one allocation each: writing one leaves the others,
+    with and without inference mode, and each outlives the rest."""
+    with torch.inference_mode(inference):
+        tab = torch.zeros(3, 4, dtype=torch.int32, device=DEV)
+        args = (_ints([2, 0, 5]), _ints([0, 16, 3]), tab, torch.arange(10, 20, dtype=torch.int32, device=DEV), 16, 9)
+        first = ops.paged_batch_plan(*args)
+        kept = [x.clone() for x in first]
+        assert [x.numel() for x in first] == [4, 3, 9, 9, 9, 1] and all(x.is_contiguous() for x in first)
+        for i, x in enumerate(first):
+            x.fill_(-9)
+            for y, z in zip(first[i + 1:], kept[i + 1:]):
+                assert torch.equal(y, z)
+        used = ops.paged_batch_plan(_ints([2, 0, 5]), _ints([0, 16, 3]), tab, args[3], 16, 9)[5]
+        torch.empty(1 << 20, device=DEV).fill_(7.0)
+        assert used.tolist() == [1]
+        same = torch.ones(3, 4, dtype=torch.int32, device=DEV)
+        starts, shared = ops.shared_prefix_groups(same, _ints([64, 64, 64]), 16, 16)
+        starts.fill_(5)
+        assert shared.tolist() == [64, 0, 0]

@@ -116,6 +116,10 @@ class AttentionVariant:
     alibi_slopes: Optional[torch.Tensor] = None
     window: int = 0
 
+    def __post_init__(self) -> None:
+        if not 0 <= self.softcap < float("inf") or self.window < 0:
+            raise ValueError(f"softcap and window must not be negative, got {self.softcap} and {self.window}")
+
     def __bool__(self) -> bool:
         return self.softcap > 0 or self.alibi_slopes is not None or self.window > 0
 
