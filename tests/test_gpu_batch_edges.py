@@ -12,7 +12,8 @@ import pytest
 import torch
 
 from test_gpu_batch_attn import DEV, DTYPES, Pools, _ints, _tables, check, run, want
-from turboquant_kv import ops
+from turboquant_kv import TurboQuantConfig, ops
+from turboquant_kv.vllm_plugin import AttentionVariant, PagedKVPools, TurboQuantAttentionMetadata
 
 pytestmark = pytest.mark.gpu
 
@@ -258,3 +259,25 @@ def test_small_results_are_tensors_of_their_own(inference):
         starts, shared = ops.shared_prefix_groups(same, _ints([64, 64, 64]), 16, 16)
         starts.fill_(5)
         assert shared.tolist() == [64, 0, 0]
+
+
+@pytest.mark.parametrize("layout", ["decode", "bitplane"])
+def test_steps_without_starts_and_on_the_host(layout):
+    """A decode step's metadata without query_start_loc means a token per sequence; queries and a
+    result on the host give what the device gives."""
+    g = torch.Generator(device=DEV).manual_seed(41)
+    pools = PagedKVPools(TurboQuantConfig(), 1, 8, 16, 2, 64, layout=layout)
+    tables = torch.arange(8, dtype=torch.int32, device=DEV).view(2, 4)
+    k, v = (torch.randn(100, 2, 64, device=DEV, generator=g) for _ in range(2))
+    t = torch.arange(100, device=DEV)
+    pools.write(0, k, v, torch.where(t < 60, t, 64 + t - 60))
+    q = torch.randn(2, 8, 64, device=DEV, generator=g)
+    variant = AttentionVariant(softcap=20.0, window=50)
+    with_starts = TurboQuantAttentionMetadata(None, _ints([60, 40]), tables, _ints([0, 1, 2]), 0)
+    without = TurboQuantAttentionMetadata(None, _ints([60, 40]), tables, None, 0)
+    ref = pools.attend(0, q, with_starts, 0.125, variant)
+    assert torch.equal(pools.attend(0, q, without, 0.125, variant), ref)
+    host = pools.attend(0, q.cpu(), without, 0.125, variant)
+    assert host.device.type == "cpu" and torch.equal(host, ref.cpu())
+    dst = torch.full((2, 8, 64), 3.0)
+    assert pools.attend(0, q, without, 0.125, variant, dst) is dst and torch.equal(dst, ref.cpu())

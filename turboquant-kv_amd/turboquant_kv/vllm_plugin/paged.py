@@ -397,6 +397,9 @@ class PagedKVPools:
         v = variant if variant is not None else AttentionVariant()
         st = self.layers[layer]
         given, q = q, q.to(self.device)
+        starts = md.query_start_loc
+        if starts is None:  # a decode step's metadata may come without: a token per sequence
+            starts = torch.arange(md.block_tables.shape[0] + 1, dtype=torch.int32, device=self.device)
         if v.alibi_slopes is not None and not v.alibi_slopes.is_cuda:
             v.alibi_slopes = v.alibi_slopes.to(self.device)  # once: later steps may be captured
         kw = dict(softcap=v.softcap, alibi_slopes=v.alibi_slopes, window=v.window,
@@ -406,11 +409,10 @@ class PagedKVPools:
             qc = q.float() if wide else q
             # (all queries are read before a row is written: the result may lie in their memory)
             direct = (output is not None and output.device == q.device and output.shape == q.shape
-                      and output.dtype == qc.dtype and output.stride()[1:] == (q.shape[2], 1) and output.data_ptr() % 16 == 0
-                      and output.stride(0) >= q.shape[1] * q.shape[2]
+                      and output.dtype == qc.dtype and output.stride()[1:] == (q.shape[2], 1)
+                      and output.data_ptr() % 16 == 0 and output.stride(0) >= q.shape[1] * q.shape[2]
                       and output.stride(0) * output.element_size() % 16 == 0)
-            args = [qc, st["kp"], st["kn"], st["vt"], st["vn"], md.block_tables, md.query_start_loc,
-                    md.seq_lens]
+            args = [qc, st["kp"], st["kn"], st["vt"], st["vn"], md.block_tables, starts, md.seq_lens]
             tail = [self.kcen, self.vcen, self.R_k, self.R_v, float(scale)]
             if direct:
                 kw["out"] = output
@@ -422,11 +424,11 @@ class PagedKVPools:
             if output is None or direct:
                 return res.to(given) if output is None else res
             # a few rows behind the last sequence keep the output's values
-            live = torch.arange(q.shape[0], device=output.device) < md.query_start_loc.to(output.device)[-1]
+            live = torch.arange(q.shape[0], device=output.device) < starts.to(output.device)[-1]
             output.copy_(torch.where(live[:, None, None], res.to(output), output))
             return output
         out = output if output is not None else torch.zeros_like(given)
-        qsl = md.query_start_loc_cpu or md.query_start_loc.tolist()
+        qsl = md.query_start_loc_cpu or starts.tolist()
         lens = md.seq_lens_cpu or md.seq_lens.tolist()
         for b, T in enumerate(lens):
             i, j = qsl[b], qsl[b + 1]
